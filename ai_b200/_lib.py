@@ -32,6 +32,7 @@ DT_BF16 = 1
 DT_F16 = 2
 
 MAX_DENSE = 4
+MAX_TOP = 64  # FG_MAX_TOP: alternatives of fg_log_probs
 
 # Phases of fg_model_read_profile (include/fgemma.h FG_PHASE_*).
 PHASES = ["embed", "gemm_qkv", "qk_norm_rope", "attention", "gemm_o", "residual",
@@ -132,6 +133,18 @@ SIGNATURES = {
     "fg_nearest": (C.c_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, C.c_int, _vp]),
     "fg_kmeans": (C.c_int, [_i64, _i64, _vp, _i64, C.c_int, C.c_int, C.c_uint64, _vp, _vp, _vp, _vp,
                             C.POINTER(C.c_int), C.c_int, _vp]),
+    "fg_embedding": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _i64, C.c_float, C.c_int, _vp, C.c_int,
+                               _i64, _vp]),
+    "fg_embedding_grad": (C.c_int, [_vp, C.c_int, _i64, _vp, _i64, _i64, _i64, C.c_float, C.c_int, _vp,
+                                    C.c_int, _i64, C.c_int, _vp]),
+    "fg_embedding_grad_rows": (C.c_int, [_vp, C.c_int, _i64, _vp, _i64, _i64, _i64, C.c_float, C.c_int, _vp,
+                                         _vp, C.c_int, _i64, _vp, _vp]),
+    "fg_log_probs": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, C.c_int, _vp, _vp, _vp, _vp,
+                               _vp, _vp]),
+    "fg_log_probs_grad": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp,
+                                    _i64, _vp]),
+    "fg_clip_grad_norm": (C.c_int, [C.c_int, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(C.c_int),
+                                    C.POINTER(_vp), C.c_float, _vp, _vp]),
 }
 
 

@@ -30,6 +30,9 @@ SOURCES = [
     "fg_noalloc.cu",
     "fg_multi.cu",
     "fg_cluster.cu",
+    "fg_embedding.cu",
+    "fg_logprobs.cu",
+    "fg_gradnorm.cu",
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

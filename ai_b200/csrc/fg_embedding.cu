@@ -1,0 +1,608 @@
+// The embedding table's operators: rows gathered by token id and scaled,
+// and the table's gradient, the sum of the gradients of the tokens that met
+// each row.
+//
+//   lookup:   y[t] = scale · W[id_t]
+//   gradient: G[v] = scale · Σ_{t : id_t = v} dy[t]
+//
+// The gradient sorts the tokens by id (a stable radix sort, so a row's
+// tokens stay in their order), cuts the sorted tokens into chunks of equal
+// length however often a token occurs, sums each chunk's runs of one id in
+// registers and joins the runs that cross chunks in a second kernel. Sums
+// are in 32 bits in an order that depends on the ids alone, so a repeated
+// call gives the same bits; a sum is rounded once, when its row is written.
+#include <algorithm>
+
+#include "fg_kernels.cuh"
+#include "fg_ptx.cuh"
+#include "fg_types.cuh"
+
+namespace fg {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+bool multiple_of(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % uintptr_t(bytes) == 0; }
+
+// Whether rows of type code dt at p with leading dimension ld hold whole
+// groups of n values, each at a multiple of its size (16 bytes at most).
+bool grouped(const void* p, int dt, int64_t dim, int64_t ld, int n) {
+  const int64_t bytes = std::min<int64_t>(16, n * dtype_size(dt));
+  return dim % n == 0 && multiple_of(p, bytes) && ld * dtype_size(dt) % bytes == 0;
+}
+
+// ---------------------------------------------------------------- lookup
+// One warp per token; a lane takes groups of VEC columns 32 groups apart.
+// Bound by memory: a row read (from L2 when it is met again) and one
+// written per token.
+constexpr int kLookupWarps = 8;
+constexpr int kLookupUnroll = 4;
+
+template <typename TW, typename TY, int VEC>
+__global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(const TW* __restrict__ table, int64_t vocab, int dim,
+                                                                  int64_t ldt, const int32_t* __restrict__ ids,
+                                                                  int64_t n, float scale, int padding,
+                                                                  TY* __restrict__ out, int64_t ldo, int* err) {
+  const int64_t t = int64_t(blockIdx.x) * kLookupWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (t >= n) return;
+  const int id = ids[t];
+  const bool pad = id == padding;
+  const bool bad = !pad && (id < 0 || id >= vocab);
+  if (bad && lane == 0) atomicCAS(err, 0, kDevBadIndex);
+  TY* y = out + t * ldo;
+  const int groups = dim / VEC;
+  if (pad || bad) {
+    Pack<TY, VEC> z;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
+    for (int c = lane; c < groups; c += 32) z.store(y + int64_t(c) * VEC);
+    return;
+  }
+  const TW* w = table + int64_t(id) * ldt;
+  for (int c0 = lane; c0 < groups; c0 += 32 * kLookupUnroll) {
+    Pack<TW, VEC> in[kLookupUnroll];
+#pragma unroll
+    for (int u = 0; u < kLookupUnroll; ++u)
+      if (c0 + 32 * u < groups) in[u].load(w + int64_t(c0 + 32 * u) * VEC);
+#pragma unroll
+    for (int u = 0; u < kLookupUnroll; ++u) {
+      if (c0 + 32 * u >= groups) break;
+      Pack<TY, VEC> r;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r.set(i, in[u].get(i) * scale);
+      r.store(y + int64_t(c0 + 32 * u) * VEC);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sort
+// Stable sort of (key, position) by the key's bits, DIGIT bits at a time
+// from the lowest: per pass the digits of each tile of tokens are counted,
+// the counts scanned digit by digit over the tiles, and every token moved to
+// its digit's place. A key is the token's id, or `vocab` (after every row)
+// for a token without a row: padding, and an id out of range.
+constexpr int kSortThreads = 256;
+constexpr int kSortItems = 16;  // a thread's tokens of a tile
+constexpr int kSortTile = kSortThreads * kSortItems;
+constexpr int kMaxDigit = 10;
+
+__device__ __forceinline__ uint32_t token_key(int id, int64_t vocab, int padding, int* err) {
+  if (id == padding) return uint32_t(vocab);
+  if (id < 0 || id >= vocab) {
+    atomicCAS(err, 0, kDevBadIndex);
+    return uint32_t(vocab);
+  }
+  return uint32_t(id);
+}
+
+// keys of the first pass from the ids (keys == nullptr), else from memory
+__device__ __forceinline__ uint32_t sort_key(const int32_t* ids, const uint32_t* keys, int64_t i, int64_t vocab,
+                                             int padding, int* err) {
+  return keys ? keys[i] : token_key(ids[i], vocab, padding, err);
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const int32_t* __restrict__ ids,
+                                                                 const uint32_t* __restrict__ keys, int64_t n,
+                                                                 int64_t vocab, int padding, int shift, int digit_bits,
+                                                                 uint32_t* __restrict__ counts, int* err) {
+  __shared__ uint32_t hist[1 << kMaxDigit];
+  const int radix = 1 << digit_bits;
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
+  __syncthreads();
+  const int64_t base = int64_t(blockIdx.x) * kSortTile;
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = base + k * kSortThreads + threadIdx.x;
+    if (i < n) atomicAdd(&hist[(sort_key(ids, keys, i, vocab, padding, err) >> shift) & (radix - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) counts[int64_t(d) * gridDim.x + blockIdx.x] = hist[d];
+}
+
+// Exclusive scan of m counts by one block, in place; the total to *total.
+constexpr int kScanThreads = 1024;
+__global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ x, int64_t m, int32_t* total) {
+  __shared__ uint32_t sums[32];
+  __shared__ uint32_t carry;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) carry = 0;
+  __syncthreads();
+  for (int64_t base = 0; base < m; base += kScanThreads) {
+    const int64_t i = base + threadIdx.x;
+    const uint32_t v = i < m ? x[i] : 0;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(kFull, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t w = sums[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(kFull, w, o);
+        if (lane >= o) w += u;
+      }
+      sums[lane] = w;
+    }
+    __syncthreads();
+    const uint32_t before = carry + (warp ? sums[warp - 1] : 0);
+    if (i < m) x[i] = before + s - v;
+    __syncthreads();
+    if (threadIdx.x == kScanThreads - 1) carry = before + s;
+    __syncthreads();
+  }
+  if (total && threadIdx.x == 0) *total = int32_t(carry);
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const int32_t* __restrict__ ids,
+                                                                const uint32_t* __restrict__ keys,
+                                                                const uint32_t* __restrict__ pos, int64_t n,
+                                                                int64_t vocab, int padding, int shift, int digit_bits,
+                                                                const uint32_t* __restrict__ counts,
+                                                                uint32_t* __restrict__ keys_out,
+                                                                uint32_t* __restrict__ pos_out, int* err) {
+  constexpr int kWarps = kSortThreads / 32;
+  __shared__ uint32_t next[kWarps][1 << kMaxDigit];  // a warp's next place for each digit
+  const int radix = 1 << digit_bits;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int d = threadIdx.x; d < radix; d += kSortThreads)
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) next[w][d] = 0;
+  __syncthreads();
+  // a warp's tokens are consecutive: 32 in each of its rounds
+  const int64_t base = int64_t(blockIdx.x) * kSortTile + int64_t(warp) * 32 * kSortItems + lane;
+  uint32_t key[kSortItems], rank[kSortItems];
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = base + 32 * k;
+    key[k] = i < n ? sort_key(ids, keys, i, vocab, padding, err) : 0;
+    const unsigned live = __ballot_sync(kFull, i < n);
+    rank[k] = 0;
+    if (i < n) {
+      const uint32_t d = (key[k] >> shift) & (radix - 1);
+      const unsigned same = __match_any_sync(live, d);
+      const uint32_t before = __popc(same & ((1u << lane) - 1));
+      rank[k] = next[warp][d] + before;
+      __syncwarp(live);
+      if (before == 0) next[warp][d] += __popc(same);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) {
+    uint32_t at = counts[int64_t(d) * gridDim.x + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t c = next[w][d];
+      next[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = base + 32 * k;
+    if (i >= n) break;
+    const uint32_t to = next[warp][(key[k] >> shift) & (radix - 1)] + rank[k];
+    keys_out[to] = key[k];
+    pos_out[to] = pos ? pos[i] : uint32_t(i);
+  }
+}
+
+// ------------------------------------------------------ the rows met
+// Number of rows whose first sorted token lies in each tile.
+__global__ void __launch_bounds__(kSortThreads) heads_count_kernel(const uint32_t* __restrict__ keys, int64_t n,
+                                                                  int64_t vocab, uint32_t* __restrict__ counts) {
+  int mine = 0;
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = int64_t(blockIdx.x) * kSortTile + k * kSortThreads + threadIdx.x;
+    const bool head = i < n && keys[i] < vocab && (i == 0 || keys[i - 1] != keys[i]);
+    mine += __syncthreads_count(head);
+  }
+  if (threadIdx.x == 0) counts[blockIdx.x] = mine;
+}
+
+// place[i] = the number of rows met before sorted token i's, row_ids its id.
+__global__ void __launch_bounds__(kSortThreads) heads_place_kernel(const uint32_t* __restrict__ keys, int64_t n,
+                                                                  int64_t vocab, const uint32_t* __restrict__ counts,
+                                                                  uint32_t* __restrict__ place,
+                                                                  int32_t* __restrict__ row_ids) {
+  __shared__ int sums[kSortThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t before = counts[blockIdx.x];
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = int64_t(blockIdx.x) * kSortTile + k * kSortThreads + threadIdx.x;
+    const bool live = i < n && keys[i] < vocab;
+    const bool head = live && (i == 0 || keys[i - 1] != keys[i]);
+    const unsigned mask = __ballot_sync(kFull, head);
+    if (lane == 0) sums[warp] = __popc(mask);
+    __syncthreads();
+    uint32_t mine = before;
+    for (int w = 0; w < kSortThreads / 32; ++w) {
+      if (w < warp) mine += sums[w];
+      before += sums[w];
+    }
+    __syncthreads();
+    mine += __popc(mask & (kFull >> (31 - lane)));  // heads up to and with this token
+    if (live) place[i] = mine - 1;
+    if (head) row_ids[mine - 1] = int32_t(keys[i]);
+  }
+}
+
+__global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* count) {
+  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i < n && i >= *count) row_ids[i] = -1;
+}
+
+// ------------------------------------------------------------------ sums
+// A warp sums one chunk of sorted tokens over 32·VEC columns, with kAhead
+// rows in flight. A run of one id that lies within the chunk is written as
+// its row; a run that came in from the chunk before leaves its sum in
+// head[chunk], one that goes on into the next chunk (and began here) in
+// tail[chunk].
+constexpr int kChunk = 32;
+constexpr int kAhead = 8;
+constexpr int kSumWarps = 8;
+
+struct SumArgs {
+  const uint32_t* keys;
+  const uint32_t* pos;
+  const uint32_t* place;  // row of the output for each sorted token; null: its key
+  int64_t n, vocab;
+  int dim, slices;
+  int64_t ldy, ldg;
+  float scale;
+  int accumulate;
+  float* head;
+  float* tail;  // [chunks, dim] each
+};
+
+template <typename TG, int VEC>
+__device__ __forceinline__ void write_row(TG* g, const float (&acc)[VEC], float scale, int accumulate) {
+  Pack<TG, VEC> r;
+  if (accumulate) {
+    r.load_own(g);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.set(i, __fadd_rn(r.get(i), __fmul_rn(acc[i], scale)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.set(i, acc[i] * scale);
+  }
+  r.store(g);
+}
+
+template <typename TY, typename TG, int VEC>
+__global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(SumArgs a, const TY* __restrict__ dy, TG* grad) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
+  const int64_t chunk = unit / a.slices;
+  const int col = (int(unit % a.slices) * 32 + lane) * VEC;
+  const int64_t i0 = chunk * kChunk;
+  if (i0 >= a.n) return;
+  const int count = int(a.n - i0 < kChunk ? a.n - i0 : kChunk);
+  const uint32_t key = lane < count ? a.keys[i0 + lane] : 0xffffffffu;
+  const uint32_t pos = lane < count ? a.pos[i0 + lane] : 0;
+  const uint32_t to = !a.place ? key : lane < count && key < a.vocab ? a.place[i0 + lane] : 0;
+  const uint32_t before = i0 > 0 ? a.keys[i0 - 1] : 0xffffffffu;
+  const uint32_t after = i0 + count < a.n ? a.keys[i0 + count] : 0xffffffffu;
+  const bool in = col < a.dim;
+  float acc[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  bool from_before = true;  // the current run is the chunk's first
+  for (int t0 = 0; t0 < count; t0 += kAhead) {
+    Pack<TY, VEC> v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int t = t0 + u;
+      const uint32_t k = __shfl_sync(kFull, key, t & 31), p = __shfl_sync(kFull, pos, t & 31);
+      if (t < count && k < a.vocab && in) v[u].load(dy + int64_t(p) * a.ldy + col);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int t = t0 + u;
+      const uint32_t k = __shfl_sync(kFull, key, t & 31), next = __shfl_sync(kFull, key, (t + 1) & 31);
+      const uint32_t row = __shfl_sync(kFull, to, t & 31);
+      if (t >= count || k >= a.vocab) return;  // tokens without a row come last
+      if (in)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
+      const bool last = t == count - 1;
+      if (last || next != k) {
+        const bool came = from_before && before == k;
+        const bool goes = last && after == k;
+        if (in) {
+          if (came || goes) {
+            float* ws = (came ? a.head : a.tail) + chunk * a.dim + col;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ws[i] = acc[i];
+          } else {
+            write_row<TG, VEC>(grad + int64_t(row) * a.ldg + col, acc, a.scale, a.accumulate);
+          }
+        }
+        from_before = false;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      }
+    }
+  }
+}
+
+// The runs that cross chunks: the chunk in which one begins adds the heads
+// of the chunks after it, in their order, and writes the row.
+template <typename TG, int VEC>
+__global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* grad) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
+  int64_t chunk = unit / a.slices;
+  const int col = (int(unit % a.slices) * 32 + lane) * VEC;
+  const int64_t i0 = chunk * kChunk, end = i0 + kChunk;
+  if (end >= a.n) return;
+  const uint32_t key = a.keys[end - 1];
+  if (key >= a.vocab || a.keys[end] != key) return;  // no run goes on
+  if (a.keys[i0] == key && i0 > 0 && a.keys[i0 - 1] == key) return;  // it began earlier
+  if (col >= a.dim) return;
+  float acc[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = a.tail[chunk * a.dim + col + i];
+  const int64_t row = a.place ? a.place[end - 1] : key;
+  while (true) {
+    ++chunk;
+    const float* h = a.head + chunk * a.dim + col;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] += h[i];
+    const int64_t next = (chunk + 1) * kChunk;
+    if (next >= a.n || a.keys[next] != key || a.keys[next - 1] != key) break;
+  }
+  write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
+}
+
+// Zeros in the rows of the dense gradient that no token met (count null;
+// there may be no tokens at all), or past the last row of the compact one:
+// a warp takes 32 rows.
+template <typename TG, int VEC>
+__global__ void __launch_bounds__(kSumWarps * 32) zero_rows_kernel(const uint32_t* __restrict__ keys, int64_t n,
+                                                                  const int32_t* __restrict__ count, TG* grad,
+                                                                  int64_t rows, int dim, int64_t ldg) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r0 = (int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5)) * 32;
+  if (r0 >= rows) return;
+  unsigned met = 0;
+  if (!count) {
+    // first sorted token with a key >= r0: each step probes 32 places
+    int64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
+    while (hi > lo) {
+      const int64_t step = (hi - lo + 31) / 32;
+      const int64_t p = lo + lane * step;
+      const bool below = p < hi && keys[p] < r0;
+      const int c = __popc(__ballot_sync(kFull, below));
+      if (c == 0) {
+        hi = lo;
+      } else {
+        const int64_t last = lo + (c - 1) * step;
+        hi = last + step < hi ? last + step : hi;
+        lo = last + 1;
+      }
+    }
+    for (int64_t i = lo; i < n; i += 32) {
+      const uint32_t k = i + lane < n ? keys[i + lane] : 0xffffffffu;
+      const bool mine = k < r0 + 32 && k >= r0;
+      met |= __reduce_or_sync(kFull, mine ? 1u << (k - r0) : 0u);
+      if (!__all_sync(kFull, mine)) break;
+    }
+  } else {
+    const int64_t c = *count;
+    met = c >= r0 + 32 ? kFull : c > r0 ? (1u << (c - r0)) - 1 : 0;
+  }
+  Pack<TG, VEC> z;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
+  for (int r = 0; r < 32 && r0 + r < rows; ++r) {
+    if (met >> r & 1) continue;
+    for (int c = lane; c < dim / VEC; c += 32) z.store(grad + (r0 + r) * ldg + int64_t(c) * VEC);
+  }
+}
+
+int64_t blocks_of(int64_t n, int64_t per) { return (n + per - 1) / per; }
+size_t round256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Scratch {
+  cudaStream_t s;
+  void* p = nullptr;
+  explicit Scratch(cudaStream_t st) : s(st) {}
+  ~Scratch() { scratch_free(p, s); }
+};
+
+// Both gradients: grad is [vocab, dim] and count null, or grad is [n, dim]
+// with row_ids [n] and the count.
+int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab, int64_t dim,
+                   float scale, int padding, void* grad, int grad_dtype, int64_t ldg, int accumulate, int32_t* row_ids,
+                   int32_t* count, cudaStream_t s) {
+  int* err = nullptr;
+  FG_TRY(device_error_word(&err));
+  const bool compact = count != nullptr;
+  if (compact && n == 0) {
+    FG_CUDA_TRY(cudaMemsetAsync(count, 0, sizeof(int32_t), s));
+    return FG_OK;
+  }
+  int bits = 1;
+  while (bits < 31 && (int64_t(1) << bits) <= vocab) ++bits;  // keys reach vocab itself
+  const int passes = (bits + kMaxDigit - 1) / kMaxDigit;
+  const int digit = (bits + passes - 1) / passes;
+  const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, kChunk);
+  const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
+  const size_t hist = round256(size_t(tiles) * (size_t(1) << digit) * 4);
+  Scratch ws(s);
+  FG_TRY(scratch_alloc(&ws.p, 5 * list + hist + 2 * part, s));
+  unsigned char* at = static_cast<unsigned char*>(ws.p);
+  auto take = [&](size_t bytes) {
+    void* r = at;
+    at += bytes;
+    return r;
+  };
+  uint32_t* key[2] = {static_cast<uint32_t*>(take(list)), static_cast<uint32_t*>(take(list))};
+  uint32_t* pos[2] = {static_cast<uint32_t*>(take(list)), static_cast<uint32_t*>(take(list))};
+  uint32_t* place = static_cast<uint32_t*>(take(list));
+  uint32_t* counts = static_cast<uint32_t*>(take(hist));
+  SumArgs a{};
+  a.head = static_cast<float*>(take(part));
+  a.tail = static_cast<float*>(take(part));
+  if (n > 0) {
+    for (int p = 0; p < passes; ++p) {
+      const uint32_t* k = p ? key[(p + 1) & 1] : nullptr;
+      sort_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, n, vocab, padding, p * digit, digit, counts, err);
+      scan_kernel<<<1, kScanThreads, 0, s>>>(counts, tiles << digit, nullptr);
+      sort_move_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, p ? pos[(p + 1) & 1] : nullptr, n, vocab, padding,
+                                                               p * digit, digit, counts, key[p & 1], pos[p & 1], err);
+    }
+  }
+  a.keys = key[(passes - 1) & 1];
+  a.pos = pos[(passes - 1) & 1];
+  a.n = n;
+  a.vocab = vocab;
+  a.dim = int(dim);
+  a.ldy = ldy;
+  a.ldg = ldg;
+  a.scale = scale;
+  a.accumulate = accumulate;
+  if (compact) {
+    heads_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts);
+    scan_kernel<<<1, kScanThreads, 0, s>>>(counts, tiles, count);
+    heads_place_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts, place, row_ids);
+    rest_ids_kernel<<<unsigned(blocks_of(n, 256)), 256, 0, s>>>(row_ids, n, count);
+    a.place = place;
+  }
+  FG_CUDA_TRY(cudaGetLastError());
+  const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
+  const int vec = wide ? 4 : 1;
+  a.slices = int(blocks_of(dim, 32 * vec));
+  const int64_t rows = compact ? n : vocab;
+  return by_dtype(grad_dtype, [&](auto tg) {
+    using TG = typename decltype(tg)::type;
+    TG* g = static_cast<TG*>(grad);
+    const unsigned zero_blocks = unsigned(blocks_of(rows, 32 * kSumWarps));
+    if (!accumulate && rows > 0) {
+      if (wide)
+        zero_rows_kernel<TG, 4><<<zero_blocks, kSumWarps * 32, 0, s>>>(a.keys, n, count, g, rows, a.dim, ldg);
+      else
+        zero_rows_kernel<TG, 1><<<zero_blocks, kSumWarps * 32, 0, s>>>(a.keys, n, count, g, rows, a.dim, ldg);
+      FG_CUDA_TRY(cudaGetLastError());
+    }
+    if (n == 0) return FG_OK;
+    const unsigned sum_blocks = unsigned(blocks_of(chunks * a.slices, kSumWarps));
+    FG_TRY(by_dtype(dy_dtype, [&](auto ty) {
+      using TY = typename decltype(ty)::type;
+      const TY* y = static_cast<const TY*>(dy);
+      if (wide)
+        sum_kernel<TY, TG, 4><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, y, g);
+      else
+        sum_kernel<TY, TG, 1><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, y, g);
+      FG_CUDA_TRY(cudaGetLastError());
+      return FG_OK;
+    }));
+    if (wide)
+      join_kernel<TG, 4><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, g);
+    else
+      join_kernel<TG, 1><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, g);
+    FG_CUDA_TRY(cudaGetLastError());
+    return FG_OK;
+  });
+}
+
+// The refusals both gradients share.
+int check_grad(const char* op, const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab,
+               int64_t dim, const void* grad, int grad_dtype, int64_t ldg, int64_t rows) {
+  if (n < 0 || vocab < 0 || dim <= 0 || n >= INT32_MAX || vocab >= INT32_MAX || dim > (1 << 20))
+    return set_error(FG_EINVAL, "%s: bad shape n=%lld vocab=%lld dim=%lld", op, (long long)n, (long long)vocab, (long long)dim);
+  if (!known_dtype(dy_dtype) || !known_dtype(grad_dtype))
+    return set_error(FG_EINVAL, "%s: unknown element type %d or %d", op, dy_dtype, grad_dtype);
+  if (ldy < dim || ldg < dim) return set_error(FG_EINVAL, "%s: leading dimension smaller than the row", op);
+  if (n > 0 && (!dy || !ids)) return set_error(FG_EINVAL, "%s: null operand", op);
+  if (!grad && rows > 0) return set_error(FG_EINVAL, "%s: null operand", op);
+  return FG_OK;
+}
+
+}  // namespace
+
+}  // namespace fg
+
+using namespace fg;
+
+extern "C" {
+
+int fg_embedding(const void* table, int table_dtype, int64_t vocab, int64_t dim, int64_t ldt, const int32_t* ids,
+                 int64_t n, float scale, int padding, void* out, int out_dtype, int64_t ldo, void* stream) {
+  clear_error();
+  if (n < 0 || vocab < 0 || dim <= 0 || n >= INT32_MAX || vocab >= INT32_MAX || dim > (1 << 20))
+    return set_error(FG_EINVAL, "fg_embedding: bad shape n=%lld vocab=%lld dim=%lld", (long long)n, (long long)vocab, (long long)dim);
+  if (!known_dtype(table_dtype) || !known_dtype(out_dtype))
+    return set_error(FG_EINVAL, "fg_embedding: unknown element type %d or %d", table_dtype, out_dtype);
+  if (ldt < dim || ldo < dim) return set_error(FG_EINVAL, "fg_embedding: leading dimension smaller than the row");
+  if (n == 0) return FG_OK;
+  if (!ids || !out || (!table && vocab > 0)) return set_error(FG_EINVAL, "fg_embedding: null operand");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int* err = nullptr;
+  FG_TRY(device_error_word(&err));
+  const unsigned blocks = unsigned(blocks_of(n, kLookupWarps));
+  const bool wide = grouped(table, table_dtype, dim, ldt, 4) && grouped(out, out_dtype, dim, ldo, 4);
+  return by_dtype(table_dtype, [&](auto tw) {
+    return by_dtype(out_dtype, [&](auto ty) {
+      using TW = typename decltype(tw)::type;
+      using TY = typename decltype(ty)::type;
+      const TW* w = static_cast<const TW*>(table);
+      TY* y = static_cast<TY*>(out);
+      if (wide)
+        lookup_kernel<TW, TY, 4><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, err);
+      else
+        lookup_kernel<TW, TY, 1><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, err);
+      FG_CUDA_TRY(cudaGetLastError());
+      return FG_OK;
+    });
+  });
+}
+
+int fg_embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab,
+                      int64_t dim, float scale, int padding, void* grad, int grad_dtype, int64_t ldg, int accumulate,
+                      void* stream) {
+  clear_error();
+  FG_TRY(check_grad("fg_embedding_grad", dy, dy_dtype, ldy, ids, n, vocab, dim, grad, grad_dtype, ldg, vocab));
+  if (vocab == 0 && n == 0) return FG_OK;
+  return embedding_grad(dy, dy_dtype, ldy, ids, n, vocab, dim, scale, padding, grad, grad_dtype, ldg, accumulate != 0,
+                        nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int fg_embedding_grad_rows(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab,
+                           int64_t dim, float scale, int padding, int32_t* row_ids, void* rows, int rows_dtype,
+                           int64_t ldr, int32_t* count, void* stream) {
+  clear_error();
+  FG_TRY(check_grad("fg_embedding_grad_rows", dy, dy_dtype, ldy, ids, n, vocab, dim, rows, rows_dtype, ldr, n));
+  if (!count || (!row_ids && n > 0)) return set_error(FG_EINVAL, "fg_embedding_grad_rows: null operand");
+  return embedding_grad(dy, dy_dtype, ldy, ids, n, vocab, dim, scale, padding, rows, rows_dtype, ldr, 0, row_ids, count,
+                        static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -26,6 +26,7 @@ enum DeviceError : int {
   kDevTimeoutAccEmpty = 4,  // MMA waited too long for the epilogue
   kDevTimeoutDrain = 5,     // teardown waited too long for in-flight work
   kDevBadArgs = 6,          // a kernel saw arguments it cannot handle
+  kDevBadIndex = 7,         // a token id or a target outside its range (reported as FG_EINVAL)
 };
 
 // Default limit of a pipeline wait, and the fixed limit of the teardown

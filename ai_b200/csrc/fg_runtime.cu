@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "fg_internal.h"
+#include "fg_ptx.cuh"
 
 namespace fg {
 
@@ -109,6 +110,8 @@ int check_device_error_word() {
       if (!first) first = v;
     }
   }
+  if (first == kDevBadIndex)
+    return set_error(FG_EINVAL, "a token id or a target was outside its range (kernel status %d)", first);
   if (first) return set_error(FG_ETIMEOUT, "a device wait gave up (kernel status %d)", first);
   return FG_OK;
 }

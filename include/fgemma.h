@@ -131,7 +131,8 @@ int fg_free(int device, void* ptr);
 int fg_memcpy_h2d(int device, void* dst, const void* src, int64_t bytes);
 int fg_memcpy_d2h(int device, void* dst, const void* src, int64_t bytes);
 /* Waits for all work on `device`; returns FG_ETIMEOUT (and clears the
- * record) when a kernel's bounded wait gave up since the last check. */
+ * record) when a kernel's bounded wait gave up since the last check, and
+ * FG_EINVAL when a training operator met an id or a target out of range. */
 int fg_synchronize(int device);
 /* Limit, in nanoseconds, of every pipeline wait (mbarrier) inside the
  * library's kernels on `device`; 0 restores the default of 2 s. A wait that
@@ -382,6 +383,70 @@ int fg_nearest(int64_t n, int64_t k, int64_t d, const float* x, int64_t ldx, con
 int fg_kmeans(int64_t n, int64_t d, const float* x, int64_t ldx, int k, int iters, uint64_t seed,
               float* centres, int32_t* assignment, float* similarity, int32_t* sizes, int* iterations,
               int precision, void* stream);
+
+/* ---- training an embedding table -----------------------------------------
+ * Device pointers; every operator is asynchronous on its stream. Values are
+ * of the given FG_DT_* type in memory, sums in 32 bits or more, each result
+ * rounded once. The reference trains on the CPU through its autograd
+ * (tensor/autograd.go); these stand for the device side of one step:
+ * lookup, loss, gradients, clipping. A token id or a target outside its
+ * range is skipped and reported by the next fg_synchronize (FG_EINVAL). */
+
+/* out[t] = scale * table[ids[t]] for n token ids and a table [vocab, dim]
+ * with row stride ldt (out: ldo, in values). A token whose id is `padding`
+ * has a zero row (a padding of -1 marks empty slots and no row of the
+ * table). table and out may have different types. */
+int fg_embedding(const void* table, int table_dtype, int64_t vocab, int64_t dim, int64_t ldt, const int32_t* ids,
+                 int64_t n, float scale, int padding, void* out, int out_dtype, int64_t ldo, void* stream);
+
+/* The table's gradient: grad[v] = scale * (sum of dy[t] over the tokens t
+ * with ids[t] == v), zero rows for the others; with accumulate != 0 the sums
+ * are added to grad and rows without a token are not touched. dy is [n, dim]
+ * (row stride ldy), grad [vocab, dim] (ldg). A row's tokens are summed in an
+ * order that depends on the ids alone: repeated calls agree bit for bit. */
+int fg_embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab,
+                      int64_t dim, float scale, int padding, void* grad, int grad_dtype, int64_t ldg, int accumulate,
+                      void* stream);
+
+/* The same gradient without the rows that no token met: row_ids[r] the ids
+ * met in ascending order, rows[r] (of [n, dim], row stride ldr) their sums,
+ * *count their number. Past the count row_ids are -1 and rows zero, so that
+ * a norm or an update may take the whole buffer without reading the count. */
+int fg_embedding_grad_rows(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab,
+                           int64_t dim, float scale, int padding, int32_t* row_ids, void* rows, int rows_dtype,
+                           int64_t ldr, int32_t* count, void* stream);
+
+/* Log probabilities over rows of logits [rows, width] (row stride ld), with
+ * z = scale * logits (scale > 0, an inverse temperature):
+ *   logprob[r] = log softmax(z_r)[targets[r]] (0 where targets[r] < 0),
+ *   entropy[r] = -sum p log p, lse[r] = log sum e^z (for the gradient),
+ * and the `top` (at most 64) most probable columns of every row in
+ * descending order, [rows, top]: equal logits by ascending index, NaN above
+ * all numbers. A row of -inf alone has log probabilities -inf and entropy 0;
+ * a row with a NaN or +inf has NaN results. */
+#define FG_MAX_TOP 64
+int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int64_t ld, const int32_t* targets,
+                 float scale, int top, float* logprob, float* entropy, float* lse, int32_t* top_index,
+                 float* top_logprob, void* stream);
+
+/* Its gradient from lse (and entropy) of fg_log_probs and the gradients of
+ * logprob and, where dentropy is not NULL, of entropy:
+ *   dlogits = scale * (dlogprob * ([j = target] - p) - dentropy * p * (log p + entropy)).
+ * A target < 0 has no part of dlogprob; a row of -inf alone has gradient 0.
+ * dlogits (row stride ldd) has the logits' type and may be the logits. */
+int fg_log_probs_grad(const void* logits, int dtype, int64_t rows, int64_t width, int64_t ld, const int32_t* targets,
+                      float scale, const float* lse, const float* entropy, const float* dlogprob,
+                      const float* dentropy, void* dlogits, int64_t ldd, void* stream);
+
+/* *norm (device) = the Euclidean norm of all values of `count` contiguous
+ * tensors (host arrays of device pointers, sizes and FG_DT_* types), and
+ * outs[i] = grads[i] * max_norm / norm where max_norm < norm < inf, else
+ * outs[i] = grads[i] (a norm that is not finite clips nothing: the caller
+ * reads it and skips its step). outs NULL = in place; outs[i] may be
+ * grads[i]. max_norm may be +inf: the norm alone. The arrays are read
+ * during the call only. */
+int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,
+                      float max_norm, float* norm, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,764 @@
+"""GPU parity of the table-training operators (ai_b200.train) against plain
+64-bit implementations, at the sizes and values where they can go wrong.
+
+Tolerances. u = 2^-24 is a float32 rounding's relative size; U[type] the
+output type's (2^-24, 2^-8, 2^-11), with its smallest step for values near
+zero. A lookup multiplies once and rounds once. A gradient row of c tokens
+is c - 1 float32 additions in some order and one product: (c + 1)·u times
+the sum of magnitudes. The softmax sums are described at ``_sum_error``.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+u = 2.0 ** -24
+TYPES = ["float32", "bfloat16", "float16"]
+U = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+TINY = {"float32": 2.0 ** -149, "bfloat16": 2.0 ** -133, "float16": 2.0 ** -24}
+
+
+def _dt(name):
+    import torch
+
+    return getattr(torch, name)
+
+
+def _name(t):
+    return str(t.dtype).replace("torch.", "")
+
+
+def _gen(cuda, seed):
+    import torch
+
+    return torch.Generator(device=cuda).manual_seed(seed)
+
+
+def _randn(shape, g, cuda, dtype="float32"):
+    import torch
+
+    return torch.randn(*shape, generator=g, device=cuda).to(_dt(dtype))
+
+
+def _near(got, want, err):
+    """|got - want| <= err plus the output type's own rounding, NaN and
+    infinities in the same places."""
+    import torch
+
+    assert got.shape == want.shape, (got.shape, want.shape)
+    k = _name(got)
+    x, y = got.double(), want.double()
+    fine = torch.isfinite(y)
+    assert torch.equal(torch.isnan(x), torch.isnan(y))
+    off = ~fine & ~torch.isnan(y)
+    assert torch.equal(x[off], y[off])
+    bound = (err if torch.is_tensor(err) else torch.full_like(y, err)) + U[k] * y.abs() * (1 + 2 * U[k]) + TINY[k]
+    d = (x - y).abs()
+    ok = ((d <= bound) | ~fine).all()
+    assert ok, (float((d - bound)[fine].max()), float(d[fine].max()), (d > bound).nonzero()[:4].tolist())
+
+
+# ------------------------------------------------------------------ lookup
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("yt", TYPES)
+@pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (5, 7, 3), (33, 100, 768), (129, 50, 769), (7, 9, 256), (1000, 2048, 132)])
+def test_lookup(cuda, wt, yt, n, vocab, dim):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n + dim)
+    w = _randn((vocab, dim), g, cuda, wt)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int32)
+    scale = dim ** 0.5
+    y = train.Embedding(w, ids, scale=scale, dtype=_dt(yt))
+    s32 = float(torch.tensor(scale, dtype=torch.float32))
+    want = w[ids.long()].double() * s32
+    _near(y, want, u * want.abs())
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("skip", [0, 1, 2, 4])
+def test_lookup_views(cuda, wt, skip):
+    """Tables that begin anywhere and whose rows are further apart than their
+    length, and a column-major one."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 3)
+    whole = _randn((40, 80), g, cuda, wt)
+    ids = torch.randint(0, 40, (3, 11), generator=g, device=cuda, dtype=torch.int32)
+    for w in (whole[:, skip:skip + 64], whole.t()[skip:, :40]):
+        got = train.Embedding(w, ids % w.shape[0])
+        assert got.shape == (3, 11, w.shape[1])
+        assert torch.equal(got, w[(ids % w.shape[0]).long()])
+
+
+def test_lookup_padding_and_empty(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    w = _randn((6, 20), _gen(cuda, 1), cuda)
+    ids = torch.tensor([0, 3, -1, 5], dtype=torch.int32, device=cuda)
+    y = train.Embedding(w, ids, padding=-1)
+    assert torch.equal(y[[0, 1, 3]], w[[0, 3, 5]]) and not y[2].any()
+    ids = torch.tensor([0, 3, 0], dtype=torch.int32, device=cuda)
+    y = train.Embedding(w, ids, padding=0)
+    assert not y[0].any() and not y[2].any() and torch.equal(y[1], w[3])
+    assert train.Embedding(w, ids[:0]).shape == (0, 20)
+    train.Check(cuda)
+
+
+def test_ids_out_of_range_are_reported(cuda):
+    """They read and write nothing; the next check names them, once."""
+    import torch
+
+    from ai_b200 import _lib, train
+
+    w = _randn((6, 8), _gen(cuda, 1), cuda)
+    ids = torch.tensor([1, 6, -2, 2 ** 31 - 1, 5], dtype=torch.int32, device=cuda)
+    y = train.Embedding(w, ids)
+    with pytest.raises(_lib.FGError) as e:
+        train.Check(cuda)
+    assert e.value.code == _lib.FG_EINVAL
+    assert not y[1:4].any() and torch.equal(y[[0, 4]], w[[1, 5]])
+    dy = torch.ones(5, 8, device=cuda)
+    for call in (lambda: train.EmbeddingGrad(dy, ids, 6), lambda: train.EmbeddingGradRows(dy, ids, 6),
+                 lambda: train.LogProbs(w, ids + 0), lambda: train.LogProbs(w, ids[:1].expand(6) + 7)):
+        try:
+            call()
+        except train.TensorError:  # five targets for six rows
+            continue
+        with pytest.raises(_lib.FGError):
+            train.Check(cuda)
+    train.Check(cuda)
+    grad = train.EmbeddingGrad(dy, ids, 6)
+    assert float(grad.sum()) == 16.0
+    with pytest.raises(_lib.FGError):
+        train.Check(cuda)
+
+
+# --------------------------------------------------------------- gradients
+def _id_patterns(n, vocab, g, cuda):
+    import torch
+
+    arange = torch.arange(n, device=cuda)
+    yield "spread", torch.randint(0, vocab, (n,), generator=g, device=cuda)
+    yield "one", torch.full((n,), vocab - 1, device=cuda)
+    yield "falling", (n - 1 - arange) % vocab
+    yield "runs", (arange // 32) % vocab
+    frequent = (vocab ** torch.rand(n, generator=g, device=cuda, dtype=torch.float64)).long() - 1
+    yield "frequent", frequent.clamp(0, vocab - 1)
+
+
+def _grad_want(dy, ids, vocab, scale, padding):
+    """(sum, error bound) of every row, in 64 bits."""
+    import torch
+
+    kept = (ids != padding) & (ids >= 0)
+    i = ids.long()[kept]
+    d = dy.double()[kept]
+    want = torch.zeros(vocab, dy.shape[1], dtype=torch.float64, device=dy.device).index_add_(0, i, d)
+    size = torch.zeros_like(want).index_add_(0, i, d.abs())
+    many = torch.zeros(vocab, dtype=torch.float64, device=dy.device).index_add_(0, i, torch.ones_like(d[:, 0]))
+    return want * scale, (many[:, None] + 1) * u * size * abs(scale) * (1 + 1e-6)
+
+
+def _check_rows(r, want, err, ids, padding):
+    import torch
+
+    kept = ids[(ids != padding) & (ids >= 0)].long()
+    met = torch.unique(kept)
+    n = len(met)
+    assert int(r.Count) == n
+    assert torch.equal(r.Ids[:n].long(), met) and bool((r.Ids[n:] == -1).all())
+    assert not r.Rows[n:].any()
+    _near(r.Rows[:n], want[met], err[met])
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (2, 3, 5), (31, 7, 64), (32, 32, 33), (33, 1023, 768), (64, 1, 128),
+                                         (1000, 1024, 130), (1025, 1025, 40), (4097, 2048, 96), (5000, 300, 769),
+                                         (20000, 262144, 64)])
+def test_grad(cuda, n, vocab, dim):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n)
+    dy = _randn((n, dim), g, cuda)
+    for what, ids in _id_patterns(n, vocab, g, cuda):
+        ids = ids.int()
+        want, err = _grad_want(dy, ids, vocab, 2.0, -1)
+        got = train.EmbeddingGrad(dy, ids, vocab, scale=2.0)
+        _near(got, want, err)
+        assert torch.equal(got, train.EmbeddingGrad(dy, ids, vocab, scale=2.0)), what
+        r = train.EmbeddingGradRows(dy, ids, vocab, scale=2.0)
+        _check_rows(r, want, err, ids, -1)
+    train.Check(cuda)
+
+
+@pytest.mark.parametrize("yt", TYPES)
+@pytest.mark.parametrize("gt", TYPES)
+@pytest.mark.parametrize("dim", [128, 65, 768])
+def test_grad_types_and_padding(cuda, yt, gt, dim):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 11)
+    n, vocab, scale = 700, 90, 0.75
+    dy = _randn((n, dim), g, cuda, yt)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int32)
+    ids[100:300] = 7
+    ids[::5] = 4
+    ids[::9] = -1
+    for padding in (-1, 4):
+        i = torch.where(ids == -1, torch.tensor(padding, dtype=torch.int32, device=cuda), ids)
+        want, err = _grad_want(dy, i, vocab, scale, padding)
+        got = train.EmbeddingGrad(dy, i, vocab, scale=scale, padding=padding, dtype=_dt(gt))
+        assert _name(got) == gt
+        _near(got, want, err)
+        r = train.EmbeddingGradRows(dy, i, vocab, scale=scale, padding=padding, dtype=_dt(gt))
+        _check_rows(r, want, err, i, padding)
+        # added to what is there; rows without a token keep their bits
+        old = _randn((vocab, dim), g, cuda, gt)
+        new = train.EmbeddingGrad(dy, i, vocab, scale=scale, padding=padding, out=old.clone(), accumulate=True)
+        sum64 = old.double() + want
+        _near(new, sum64, err + u * (want.abs() + sum64.abs()))
+        still = want.abs().sum(1) == 0
+        assert torch.equal(new[still], old[still]) and (padding != 4 or bool(still[4]))
+
+
+def test_grad_of_nothing(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    dy = torch.ones(50, 12, device=cuda)
+    pads = torch.zeros(50, dtype=torch.int32, device=cuda)
+    assert not train.EmbeddingGrad(dy, pads, 40, padding=0).any()
+    r = train.EmbeddingGradRows(dy, pads, 40, padding=0)
+    assert int(r.Count) == 0 and bool((r.Ids == -1).all()) and not r.Rows.any()
+    assert not train.EmbeddingGrad(dy[:0], pads[:0], 40).any()
+    assert train.EmbeddingGrad(dy[:0], pads[:0], 0).shape == (0, 12)
+    r = train.EmbeddingGradRows(dy[:0], pads[:0], 40)
+    assert int(r.Count) == 0 and r.Rows.shape == (0, 12) and r.Ids.shape == (0,)
+    out = torch.ones(40, 12, device=cuda)
+    assert train.EmbeddingGrad(dy[:0], pads[:0], 40, out=out, accumulate=True).eq(1).all()
+
+
+@pytest.mark.parametrize("yt", TYPES)
+def test_grad_views(cuda, yt):
+    """Gradients with 3 dimensions, rows apart, an odd start, columns first,
+    and an output with rows apart whose gaps stay as they are."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 5)
+    whole = _randn((70, 100), g, cuda, yt)
+    ids = torch.randint(0, 20, (70,), generator=g, device=cuda, dtype=torch.int32)
+    for dy in (whole[:, 1:65], whole[:, 4:36], whole.t().contiguous().t()[:, :31]):
+        want, err = _grad_want(dy, ids, 20, 1.0, -1)
+        _near(train.EmbeddingGrad(dy, ids, 20), want, err)
+        three = dy.reshape(7, 10, -1)
+        _near(train.EmbeddingGrad(three, ids.view(7, 10), 20), want, err)
+        buf = torch.full((20, dy.shape[1] + 3), 9.0, device=cuda)
+        train.EmbeddingGrad(dy, ids, 20, out=buf[:, :dy.shape[1]])
+        _near(buf[:, :dy.shape[1]], want, err)
+        assert buf[:, dy.shape[1]:].eq(9).all()
+
+
+def test_grad_wide_keys_and_many_tokens(cuda):
+    """Ids of 21 to 31 bits, and more tokens than one group of blocks sorts."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 6)
+    n = 300000
+    dy = _randn((n, 4), g, cuda)
+    for vocab in (1 << 20, (1 << 20) + 3, 2 ** 31 - 2):
+        ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int64).int()
+        ids[::3] = vocab - 1
+        ids[1::7] = 0
+        r = train.EmbeddingGradRows(dy, ids, vocab)
+        met, at = torch.unique(ids.long(), return_inverse=True)
+        want = torch.zeros(len(met), 4, dtype=torch.float64, device=cuda).index_add_(0, at, dy.double())
+        size = torch.zeros_like(want).index_add_(0, at, dy.double().abs())
+        many = torch.bincount(at).double()
+        assert int(r.Count) == len(met) and torch.equal(r.Ids[:len(met)].long(), met)
+        _near(r.Rows[:len(met)], want, (many[:, None] + 1) * u * size)
+        assert not r.Rows[len(met):].any()
+
+
+def test_offsets_past_32_bits(cuda):
+    """A table and a gradient whose last rows lie past 2^31 values."""
+    import torch
+
+    from ai_b200 import train
+
+    vocab, dim = 2_900_000, 768
+    table = torch.zeros(vocab, dim, dtype=torch.bfloat16, device=cuda)
+    table[-3:] = 2.0
+    ids = torch.tensor([vocab - 1, 5, vocab - 3], dtype=torch.int32, device=cuda)
+    y = train.Embedding(table, ids, scale=3.0)
+    assert y[[0, 2]].eq(6).all() and not y[1].any()
+    dy = torch.ones(3, dim, dtype=torch.bfloat16, device=cuda)
+    got = train.EmbeddingGrad(dy, ids, vocab, out=table.fill_(7.0))
+    assert got[[vocab - 1, vocab - 3, 5]].eq(1).all()
+    assert float(got[-4:].float().sum()) == 2 * dim and float(got[:6].float().sum()) == dim
+    assert int(got[: vocab // 2].count_nonzero()) + int(got[vocab // 2:].count_nonzero()) == 3 * dim
+    # the same places as token gradients
+    ids = torch.full((vocab,), -1, dtype=torch.int32, device=cuda)
+    ids[-2:] = 1
+    ids[4] = 0
+    table.fill_(0)
+    table[-2:] = 1.5
+    table[4] = 0.25
+    got = train.EmbeddingGrad(table, ids, 2, dtype=torch.float32)
+    assert got[1].eq(3).all() and got[0].eq(0.25).all()
+
+
+def test_operators_follow_their_stream(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 8)
+    side = torch.cuda.Stream(cuda)
+    dy = _randn((50000, 256), g, cuda)
+    ids = torch.randint(0, 5000, (50000,), generator=g, device=cuda, dtype=torch.int32)
+    want = train.EmbeddingGrad(dy, ids, 5000)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            late = torch.empty_like(dy).fill_(9.0)  # the operator must wait for what its stream does
+            late.copy_(dy)
+            got = train.EmbeddingGrad(late, ids, 5000)
+            rows = train.EmbeddingGradRows(late, ids, 5000)
+            norm = train.ClipGradNorm([got.clone()], 1.0)
+    side.synchronize()
+    assert torch.equal(got, want)
+    n = int(rows.Count)
+    assert torch.equal(rows.Rows[:n], want[rows.Ids[:n].long()])
+    assert abs(float(norm) - float(want.double().norm())) <= 1e-6 * float(norm)
+
+
+# ------------------------------------------------------- log probabilities
+def _sum_error(width, entropy):
+    """Relative error of s1 = Σ e^d. A term's d = (x − m)·scale has two
+    roundings and the exponential's argument (a product with log2 e, itself
+    rounded) two more, 4u·|d| in all, and the exponential at most 4u of its own; Σ e^d·|d| / s1 is at most the entropy.
+    The additions: at most width / 64 + 32 in a row."""
+    return u * (4 * entropy + 4 + width / 64 + 32)
+
+
+def _logprobs_want(x, t, scale):
+    import torch
+
+    z = x.double() * scale
+    m = z.amax(1, keepdim=True)
+    empty = (z == -math.inf).all(1)
+    d = z - torch.where(empty[:, None], torch.zeros_like(m), m)
+    e = torch.exp(d)
+    s1 = e.sum(1)
+    s2 = torch.where(e == 0, torch.zeros_like(d), e * d).sum(1)
+    logs = torch.log(s1)
+    dt = d.gather(1, t.long().clamp(min=0)[:, None])[:, 0]
+    logp = torch.where(empty, torch.full_like(logs, -math.inf), dt - logs)
+    logp = torch.where(t < 0, torch.zeros_like(logp), logp)
+    H = torch.where(empty, torch.zeros_like(logs), logs - s2 / s1)
+    lse = m[:, 0] + logs
+    lse = torch.where(empty, torch.full_like(logs, -math.inf), lse)
+    return d, logs, s2 / s1, logp, H, lse, empty
+
+
+def _check_logprobs(x, t, scale, top):
+    """LogProbs of x against 64 bits; the alternatives against a stable sort."""
+    import torch
+
+    from ai_b200 import train
+
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    r = train.LogProbs(x, t, scale=scale, top=top)
+    d, logs, mean, logp, H, lse, empty = _logprobs_want(x, t, scale)
+    fin = lambda v: torch.where(torch.isfinite(v), v, torch.zeros_like(v))  # noqa: E731
+    tol = _sum_error(x.shape[1], fin(H).clamp(min=0)) + u * fin(logs).abs() * 2
+    dt = fin(d.gather(1, t.long().clamp(min=0)[:, None])[:, 0])
+    _near(r.LogProb, logp, tol + u * (3 * dt.abs() + fin(logp).abs()))
+    _near(r.LogSum, lse, tol + u * (fin(lse) - fin(logs)).abs() * 2)
+    _near(r.Entropy, H, tol * (2 + 2 * fin(mean).abs()) + 2 * u * fin(mean).abs() + tol * fin(mean).abs())
+    if top:
+        value, index = x.float().sort(dim=1, descending=True, stable=True)
+        assert torch.equal(r.TopIndex.long(), index[:, :top])
+        dk = d.gather(1, index[:, :top])
+        want = torch.where(empty[:, None], torch.full_like(dk, -math.inf), dk - logs[:, None])
+        _near(r.TopLogProb, want, tol[:, None] + u * (3 * fin(dk).abs() + fin(want).abs()))
+    else:
+        assert r.TopIndex is None and r.TopLogProb is None
+    return r
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,top", [(1, 1, 1), (3, 2, 2), (5, 31, 7), (4, 33, 33), (7, 64, 64), (2, 257, 20),
+                                            (33, 1000, 8), (9, 4097, 64), (300, 513, 3), (2, 30011, 20), (1, 262144, 20),
+                                            (1, 100003, 64), (150, 8192, 8), (40, 12288, 1), (3, 70000, 0)])
+def test_logprobs(cuda, dtype, rows, width, top):
+    import torch
+
+    g = _gen(cuda, width)
+    x = _randn((rows, width), g, cuda, dtype) * 3
+    t = torch.randint(0, width, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    t[rows // 2:rows // 2 + rows // 3] = -1
+    _check_logprobs(x, t, 1.0, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,pad,skip", [(100, 1, 0), (1001, 7, 3), (4096, 8, 0), (4096, 3, 1), (20000, 5, 2)])
+def test_logprobs_views(cuda, dtype, width, pad, skip):
+    """Rows that begin anywhere, and columns first."""
+    import torch
+
+    g = _gen(cuda, width + pad)
+    buf = _randn((6, width + pad + skip), g, cuda, dtype)
+    t = torch.randint(0, width, (6,), generator=g, device=cuda, dtype=torch.int32)
+    _check_logprobs(buf[:, skip:skip + width], t, 10.0, 5)
+    if width < 2000:
+        _check_logprobs(buf[:, skip:skip + width].t().contiguous().t(), t, 10.0, 5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [40, 1500, 9000, 66000])
+def test_logprobs_orders_and_ties(cuda, dtype, width):
+    """Rising and falling rows, equal values, both zeros, few distinct values."""
+    import torch
+
+    g = _gen(cuda, width)
+    top = min(64, width)
+    up = torch.arange(width, device=cuda, dtype=torch.float32) / width
+    few = torch.randint(0, 3, (width,), generator=g, device=cuda).float()
+    zeros = torch.where(few > 1, torch.tensor(-0.0, device=cuda), torch.tensor(0.0, device=cuda))
+    late = torch.zeros(width, device=cuda)
+    late[-5:] = 1
+    x = torch.stack([up, up.flip(0), torch.full_like(up, 2.5), few, zeros, late, -late]).to(_dt(dtype))
+    t = torch.arange(7, device=cuda, dtype=torch.int32)
+    _check_logprobs(x, t, 1.0, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [7, 600, 5000, 40000])
+def test_logprobs_masked_and_not_finite(cuda, dtype, width):
+    """Masks of -inf and of the type's lowest value, rows with nothing left,
+    rows with one entry left, NaN and +inf."""
+    import torch
+
+    inf, low = math.inf, torch.finfo(_dt(dtype)).min
+    x = _randn((12, width), _gen(cuda, width), cuda, dtype)
+    x[0, ::2] = -inf
+    x[1] = -inf
+    x[2] = -inf
+    x[2, width - 1] = 1.0
+    x[3] = low
+    x[4, 1:] = low
+    x[5, 3] = math.nan
+    x[6, 2] = inf
+    x[7] = math.nan
+    x[8, :width // 2] = -inf
+    x[9] = -inf
+    x[9, 5] = math.nan
+    x[10, :] = inf
+    x[11, 1:] = -inf
+    t = torch.full((12,), 3, dtype=torch.int32, device=cuda)
+    t[2] = width - 1
+    t[8] = 0
+    r = _check_logprobs(x, t, 1.0, 5)
+    assert r.LogProb[1] == -inf and r.Entropy[1] == 0 and r.TopIndex[1].tolist() == [0, 1, 2, 3, 4]
+    assert torch.isnan(r.LogProb[5]) and torch.isnan(r.LogSum[6]) and torch.isnan(r.Entropy[7])
+
+
+def test_logprobs_past_32_bits(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    rows, width = 33000, 66000
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=cuda)
+    x[-1, 7] = 20.0
+    x[-2, width - 1] = 30.0
+    t = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    t[-1], t[-2] = 7, width - 1
+    r = train.LogProbs(x, t, top=1)
+    assert r.TopIndex[-2:, 0].tolist() == [width - 1, 7] and not r.TopIndex[:-2].any()
+    logp = 20.0 - math.log(math.exp(20.0) + width - 1)
+    assert abs(float(r.LogProb[-1]) - logp) <= 2e-3 * abs(logp) + 1e-6
+    train.LogProbsGrad(x, t, r.LogSum, torch.ones(rows, device=cuda), out=x)
+    p = math.exp(-math.log(width))
+    got = x[0].double()
+    assert abs(float(got[0]) - (1 - p)) < 2 ** -8 and abs(float(got[1]) + p) < p * 2 ** -8
+    last = x[-1].double()
+    e = width / math.exp(20.0)
+    assert abs(float(last[7]) - e) < 0.05 * e and abs(float(last[6]) + math.exp(-20.0)) < 0.01 * math.exp(-20.0)
+
+
+def _grad_rows_want(x, t, lse, H, dl, dh, scale):
+    """(gradient, error bound): p = e^(z − lse) has the relative error of its
+    argument, 4u(|z| + |lse|), the exponential's 4u and the entropy factor's."""
+    import torch
+
+    z = x.double() * scale
+    lse, dl = lse.double()[:, None], dl.double()[:, None]
+    empty = lse == -math.inf
+    logp = z - torch.where(empty, torch.zeros_like(lse), lse)
+    p = torch.exp(logp)
+    rel = 4 * u * (torch.where(p == 0, torch.zeros_like(z), z).abs() + lse.abs()) + 6 * u
+    hit = torch.zeros_like(p)
+    at = torch.arange(len(t), device=x.device)[t >= 0]
+    hit[at, t.long()[t >= 0]] = 1
+    dl = torch.where(t[:, None] < 0, torch.zeros_like(dl), dl)
+    want = dl * (hit - p)
+    err = dl.abs() * (p * rel + 2 * u * (hit + p))
+    if dh is not None:
+        dh, H = dh.double()[:, None], H.double()[:, None]
+        f = torch.where(p == 0, torch.zeros_like(p), logp + H)
+        want = want - dh * p * f
+        err = err + dh.abs() * p * (f.abs() * (rel + 4 * u) + 2 * u * (torch.where(p == 0, torch.zeros_like(z), z).abs() + lse.abs() + H.abs()))
+    zero = torch.zeros_like(want)
+    want = torch.where(empty, zero, want * scale)
+    err = torch.where(empty, zero, (err + 3 * u * want.abs() / scale) * scale)
+    # below the exponential's smallest normal result float32 gives 0
+    return want, torch.nan_to_num(err, nan=0.0) + scale * 2.0 ** -125 * (dl.abs().amax() + 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,pad", [(1, 1, 0), (3, 5, 0), (17, 33, 1), (4, 1024, 0), (5, 4099, 5), (3, 30011, 0),
+                                            (1, 262144, 0), (200, 800, 8)])
+@pytest.mark.parametrize("scale,with_entropy", [(1.0, False), (1.0, True), (20.0, True)])
+def test_logprobs_grad(cuda, dtype, rows, width, pad, scale, with_entropy):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, rows + width)
+    buf = _randn((rows, width + pad), g, cuda, dtype) * (3 / scale)
+    x = buf[:, :width]
+    if rows > 3:
+        x[1] = -math.inf
+        x[2, ::3] = -math.inf
+        x[3] = torch.finfo(_dt(dtype)).min
+    t = torch.randint(0, width, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    if rows > 1:
+        t[0] = -1
+    _, _, _, _, H, lse, _ = _logprobs_want(x, t, scale)
+    H, lse = H.float(), lse.float()
+    dl, dh = torch.randn(rows, generator=g, device=cuda), torch.randn(rows, generator=g, device=cuda)
+    dh = dh if with_entropy else None
+    want, err = _grad_rows_want(x, t, lse, H, dl, dh, scale)
+    kept = buf.clone()
+    got = train.LogProbsGrad(x, t, lse, dl, entropy=H, dentropy=dh, scale=scale)
+    assert torch.equal(buf.view(torch.uint8) if buf.is_contiguous() else buf, kept.view(torch.uint8)) and _name(got) == dtype
+    _near(got, want, err)
+    # in place, the values between the rows untouched
+    train.LogProbsGrad(x, t, lse, dl, entropy=H, dentropy=dh, scale=scale, out=x)
+    assert torch.equal(x, got) and torch.equal(buf[:, width:], kept[:, width:])
+
+
+def test_logprobs_grad_not_finite(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    x = torch.zeros(3, 700, device=cuda)
+    x[0, 4] = math.nan
+    x[1, 5] = math.inf
+    t = torch.zeros(3, dtype=torch.int32, device=cuda)
+    r = train.LogProbs(x, t)
+    got = train.LogProbsGrad(x, t, r.LogSum, torch.ones(3, device=cuda))
+    assert torch.isnan(got[:2]).all() and torch.isfinite(got[2]).all()
+
+
+def test_logprobs_grad_against_differences(cuda):
+    """The step of the loss along every logit, from 64-bit losses."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 77)
+    rows, width, scale, h = 4, 23, 3.0, 1e-4
+    x = _randn((rows, width), g, cuda)
+    t = torch.tensor([1, 22, -1, 9], dtype=torch.int32, device=cuda)
+    dl, dh = torch.randn(rows, generator=g, device=cuda), torch.randn(rows, generator=g, device=cuda)
+
+    def loss(z):  # [.., rows, width]
+        logp = torch.log_softmax(z * scale, -1)
+        H = -(logp.exp() * logp).sum(-1)
+        picked = logp.gather(-1, t.long().clamp(min=0)[:, None].expand(*z.shape[:-1], 1))[..., 0]
+        return (torch.where(t < 0, torch.zeros_like(picked), picked) * dl.double() + H * dh.double()).sum(-1)
+
+    step = h * torch.eye(rows * width, dtype=torch.float64, device=cuda).view(-1, rows, width)
+    want = ((loss(x.double() + step) - loss(x.double() - step)) / (2 * h)).view(rows, width)
+    r = train.LogProbs(x, t, scale=scale)
+    got = train.LogProbsGrad(x, t, r.LogSum, dl, entropy=r.Entropy, dentropy=dh, scale=scale).double()
+    # third derivatives of size scale^3 · |weights|: h²·27/6, and float32
+    assert float((got - want).abs().max()) <= 27 * h * h * 8 + 64 * u * scale * 8
+
+
+def test_embedding_grad_against_differences(cuda):
+    """The lookup is linear: the loss's difference along a row is its gradient."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 78)
+    w, dy = _randn((5, 6), g, cuda), _randn((40, 6), g, cuda)
+    ids = torch.randint(0, 5, (40,), generator=g, device=cuda, dtype=torch.int32)
+    got = train.EmbeddingGrad(dy, ids, 5, scale=3.0).double()
+
+    def loss(w):
+        return float((train.Embedding(w, ids, scale=3.0).double() * dy.double()).sum())
+
+    for v in range(5):
+        for c in range(6):
+            step = torch.zeros_like(w)
+            step[v, c] = 0.5
+            diff = loss(w + step) - loss(w - step)
+            assert abs(diff - float(got[v, c])) <= 40 * 8 * u * 3 * 4 * 40
+
+
+# ---------------------------------------------------------------- clipping
+def _clip_want(grads, max_norm):
+    total = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads))
+    c = max_norm / total if math.isfinite(total) and total > max_norm else 1.0
+    return total, [g.double() * c for g in grads], c
+
+
+@pytest.mark.parametrize("types", [("float32",), ("bfloat16",), ("float16",), ("float32", "bfloat16", "float16")])
+@pytest.mark.parametrize("sizes", [(1,), (3, 0, 5), (768, 768 * 768, 1, 256), (8191, 8192, 8193, 100001), tuple(range(1, 40))])
+@pytest.mark.parametrize("max_norm", [1e-3, 1e6])
+def test_clip(cuda, types, sizes, max_norm):
+    """In place and apart, in one buffer so that tensors begin anywhere."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, sum(sizes))
+    bufs = {k: _randn((sum(sizes) + 1,), g, cuda, k) for k in types}
+    grads, at = [], 1
+    for i, n in enumerate(sizes):
+        grads.append(bufs[types[i % len(types)]][at:at + n])
+        at += n
+    norm, want, c = _clip_want(grads, max_norm)
+    outs = [torch.empty_like(x) for x in grads]
+    kept = [x.clone() for x in grads]
+    got = train.ClipGradNorm(grads, max_norm, out=outs)
+    assert got.dtype == torch.float32 and got.dim() == 0 and abs(float(got) - norm) <= 4 * u * norm
+    for o, w, x, k in zip(outs, want, grads, kept):
+        _near(o, w, 4 * u * w.abs())
+        assert torch.equal(x, k)
+        if c == 1.0:
+            assert torch.equal(o, k)
+    again = train.ClipGradNorm(grads, max_norm)
+    assert float(again) == float(got)
+    for x, o in zip(grads, outs):
+        assert torch.equal(x, o)
+
+
+def test_clip_many_tensors(cuda):
+    """More tensors than one launch takes."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 2)
+    grads = [_randn((1 + i % 70,), g, cuda, TYPES[i % 3]) for i in range(2345)]
+    norm, want, _ = _clip_want(grads, 1.5)
+    got = train.ClipGradNorm(grads, 1.5)
+    assert abs(float(got) - norm) <= 4 * u * norm
+    for x, w in zip(grads, want):
+        _near(x, w, 4 * u * w.abs())
+
+
+def test_clip_extremes(cuda):
+    """Squares past float32's range, norms that are not finite, zeros, a
+    limit of 0 and of infinity."""
+    import torch
+
+    from ai_b200 import train
+
+    big = torch.full((1000,), 1e30, device=cuda)
+    got = train.ClipGradNorm([big], 1.0)
+    assert abs(float(got) / (1e30 * math.sqrt(1000)) - 1) < 4 * u
+    assert abs(float(big[0]) * math.sqrt(1000) - 1) < 8 * u
+    small = torch.full((1000,), 1e-30, device=cuda)
+    assert abs(float(train.ClipGradNorm([small], 1.0)) / (1e-30 * math.sqrt(1000)) - 1) < 4 * u
+    for bad in (math.nan, math.inf, -math.inf):
+        x = torch.ones(5000, device=cuda)
+        x[4321] = bad
+        kept = x.clone()
+        got = float(train.ClipGradNorm([x], 1.0))
+        assert (math.isnan(got) if math.isnan(bad) else got == math.inf)
+        assert torch.equal(x.nan_to_num(7.0), kept.nan_to_num(7.0))
+    z = torch.zeros(100, device=cuda)
+    assert float(train.ClipGradNorm([z], 1.0)) == 0 and not z.any()
+    x = torch.ones(100, device=cuda)
+    assert float(train.ClipGradNorm([x], math.inf)) == 10 and x.eq(1).all()
+    assert float(train.ClipGradNorm([x], 0.0)) == 10 and not x.any()
+    assert float(train.ClipGradNorm([x[:0]], 1.0)) == 0
+
+
+def test_clip_past_32_bits(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    x = torch.zeros((1 << 31) + 5, dtype=torch.bfloat16, device=cuda)
+    x[-1] = 3.0
+    x[1] = 4.0
+    assert float(train.ClipGradNorm([x], 1.0)) == 5.0
+    assert abs(float(x[-1]) - 0.6) <= 0.6 * 2 ** -8 and abs(float(x[1]) - 0.8) <= 0.8 * 2 ** -8
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    x = torch.zeros(4, 8, device=cuda)
+    i = torch.zeros(4, dtype=torch.int32, device=cuda)
+    f = torch.zeros(4, device=cuda)
+    bad = [
+        lambda: train.Embedding(x.double(), i),
+        lambda: train.Embedding(x[0], i),
+        lambda: train.Embedding(x, i.long()),
+        lambda: train.Embedding(x, i.cpu()),
+        lambda: train.Embedding(x, i, dtype=torch.float64),
+        lambda: train.EmbeddingGrad(x, i[:3], 5),
+        lambda: train.EmbeddingGrad(x, i, -1),
+        lambda: train.EmbeddingGrad(x, i, 5, accumulate=True),
+        lambda: train.EmbeddingGrad(x, i, 5, out=torch.zeros(4, 8, device=cuda)),
+        lambda: train.EmbeddingGrad(x, i, 5, out=torch.zeros(8, 5, device=cuda).t()),
+        lambda: train.EmbeddingGrad(x, i, 5, dtype=torch.float16, out=torch.zeros(5, 8, device=cuda)),
+        lambda: train.EmbeddingGradRows(x, i.long(), 5),
+        lambda: train.LogProbs(x, i, top=9),
+        lambda: train.LogProbs(x, i, top=-1),
+        lambda: train.LogProbs(torch.zeros(4, 100, device=cuda), i, top=65),
+        lambda: train.LogProbs(x, i, scale=0.0),
+        lambda: train.LogProbs(x, i[:2]),
+        lambda: train.LogProbs(x[:, :0], i),
+        lambda: train.LogProbsGrad(x, i, f[:3], f),
+        lambda: train.LogProbsGrad(x, i, f, f, dentropy=f),
+        lambda: train.LogProbsGrad(x, i, f, f.double()),
+        lambda: train.LogProbsGrad(x, i, f, f, out=x.half()),
+        lambda: train.ClipGradNorm([x.t()], 1.0),
+        lambda: train.ClipGradNorm([x, x.cpu()], 1.0),
+        lambda: train.ClipGradNorm([x], 1.0, out=[]),
+        lambda: train.ClipGradNorm([x], math.nan),
+        lambda: train.ClipGradNorm([i], 1.0),
+    ]
+    for call in bad:
+        with pytest.raises(train.TensorError):
+            call()
