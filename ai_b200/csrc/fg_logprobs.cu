@@ -78,18 +78,6 @@ struct RowSums {
     s2 = c == 0.f ? 0.f : c * fmaf(d, s1, s2);
     s1 = c == 0.f ? 0.f : c * s1;
   }
-  __device__ __forceinline__ void add(RowSums o, float k) {
-    if (o.s1 == 0.f) return;
-    if (s1 == 0.f) {
-      *this = o;
-      return;
-    }
-    const float to = max_nan(ref, o.ref);
-    move(to, k);
-    o.move(to, k);
-    s1 += o.s1;
-    s2 += o.s2;
-  }
 };
 
 // One pass over each row by the blocks of a cluster (one block where there
@@ -140,6 +128,34 @@ __device__ __forceinline__ int rank_list(RowShared<THREADS>& sh, int n, int top)
   return n;
 }
 
+// sum += x, keeping in `lost` what the sum's rounding put in too much
+// (Kahan's summation): a long row's many small terms count beside a large one.
+__device__ __forceinline__ void add_kept(float& sum, float& lost, float x) {
+  const float y = __fsub_rn(x, lost);
+  const float to = __fadd_rn(sum, y);
+  lost = __fsub_rn(__fsub_rn(to, sum), y);
+  sum = to;
+}
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(kFull));
+  return r;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+// The sums of all lanes together, in every lane. A lane that has met nothing
+// above −∞ has the reference −∞ and sums of 0.
+__device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
+  v.move(warp_max_nan(v.ref), k);
+  v.s1 = warp_sum(v.s1);
+  v.s2 = warp_sum(v.s2);
+  return v;
+}
+
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t key) {
   const uint32_t hi = __reduce_max_sync(kFull, uint32_t(key >> 32));
@@ -164,14 +180,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   const float k = a.scale * kLog2e;
   // column of a thread's entry i of a tile
   auto column = [&](int tile, int i) {
-    return (int64_t(tile) * (THREADS * G) + (i / V) * THREADS + threadIdx.x) * V - skip + i % V;
+    return (tile * (THREADS * G) + (i / V) * THREADS + int(threadIdx.x)) * V - skip + i % V;
   };
 
   Pack<T, V> next[G];
   auto load = [&](int tile) {
+    const int first = tile * (THREADS * kItems) - skip;
+    if (first >= 0 && first + THREADS * kItems <= a.width) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) next[g].load(x + column(tile, g * V));
+      return;
+    }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int64_t j = column(tile, g * V);
+      const int j = column(tile, g * V);
       if (j >= 0 && j + V <= a.width) {
         next[g].load(x + j);
       } else {  // a row's first or last group, or none of it
@@ -191,6 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   }
   if (threadIdx.x == 0) sh.count = 0;
   RowSums sums{-INFINITY, 0.f, 0.f};
+  float lost1 = 0.f, lost2 = 0.f;  // what rounding added to the sums too much
   int n = 0;                // entries of the list
   uint64_t bound = 0;       // `top` entries met reach this key
   float bound_value = NAN;  // and this value; NaN: no bound yet
@@ -205,15 +228,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 #pragma unroll
     for (int i = 1; i < kItems; ++i) most = max_nan(most, v[i]);
     const float higher = max_nan(sums.ref, most);
-    if (!(higher == sums.ref)) sums.move(higher, k);
+    if (!(higher == sums.ref)) {
+      sums.s1 -= lost1;
+      sums.s2 -= lost2;
+      lost1 = lost2 = 0.f;
+      sums.move(higher, k);
+    }
     const float ref = sums.ref == -INFINITY ? 0.f : sums.ref;
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const float d = max_nan(v[i] - ref, -FLT_MAX);  // −∞ times e^−∞ = 0 would be no number
       const float e = ex2_approx(d * k);
-      sums.s1 += e;
-      sums.s2 = fmaf(e, d, sums.s2);
+      s1 += e;
+      s2 = fmaf(e, d, s2);
     }
+    add_kept(sums.s1, lost1, s1);
+    add_kept(sums.s2, lost2, s2);
     if (a.top == 0) continue;
 
     if (tile == part) {
@@ -233,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       if (least) bound_value = rank_value(least);
     }
     auto key_of = [&](int i) {
-      const int64_t j = column(tile, i);
+      const int j = column(tile, i);
       const uint64_t key = j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
       return key > bound ? key : 0;
     };
@@ -288,26 +319,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     }
   }
 
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    RowSums other{__shfl_xor_sync(kFull, sums.ref, o), __shfl_xor_sync(kFull, sums.s1, o), __shfl_xor_sync(kFull, sums.s2, o)};
-    sums.add(other, k);
+  const RowSums none{-INFINITY, 0.f, 0.f};
+  sums.s1 -= lost1;
+  sums.s2 -= lost2;
+  sums = warp_join(sums, k);
+  if (kWarps > 1) {
+    if (lane == 0) sh.warp_sums[warp] = sums;
+    __syncthreads();
+    sums = warp_join(lane < kWarps ? sh.warp_sums[lane % kWarps] : none, k);
   }
-  if (lane == 0) sh.warp_sums[warp] = sums;
   if (a.top) n = rank_list(sh, n, a.top);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) sums.add(sh.warp_sums[w], k);
-    sh.sums = sums;
-  }
   if (split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) sh.sums = sums;
     cluster.sync();
     if (part == 0) {
-      if (threadIdx.x == 0) {
-        for (int p = 1; p < split; ++p) sums.add(cluster.map_shared_rank(&sh, p)->sums, k);
-        sh.sums = sums;
-      }
+      sums = warp_join(lane < split ? cluster.map_shared_rank(&sh, lane % split)->sums : none, k);
       // as many parts' lists at a time as the list has room for
       const int batch = a.top ? kListSize / a.top : split;
       for (int p0 = 1; a.top && p0 < split; p0 += batch) {
@@ -324,14 +351,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     cluster.sync();  // the parts' shared memory is read until here
     if (part) return;
   }
-  __syncthreads();
-  const RowSums all = sh.sums;
-  const bool empty = all.s1 == 0.f;
-  const float ref = empty ? 0.f : all.ref, logs = logf(all.s1);
+  const bool empty = sums.s1 == 0.f;
+  const float ref = empty ? 0.f : sums.ref, logs = logf(sums.s1);
   if (threadIdx.x == 0) {
-    const bool none = t < 0 || t >= a.width;
-    a.logprob[row] = none ? 0.f : empty ? -INFINITY : fmaf(xt - ref, a.scale, -logs);
-    a.entropy[row] = empty ? 0.f : logs - a.scale * (all.s2 / all.s1);
+    const bool skipped = t < 0 || t >= a.width;
+    a.logprob[row] = skipped ? 0.f : empty ? -INFINITY : fmaf(xt - ref, a.scale, -logs);
+    a.entropy[row] = empty ? 0.f : logs - a.scale * (sums.s2 / sums.s1);
     a.lse[row] = fmaf(ref, a.scale, logs);
   }
   for (int i = threadIdx.x; i < a.top; i += THREADS) {
@@ -480,7 +505,7 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
                  float scale, int top, float* logprob, float* entropy, float* lse, int32_t* top_index,
                  float* top_logprob, void* stream) {
   clear_error();
-  if (rows < 0 || width <= 0 || rows >= INT32_MAX || width >= INT32_MAX)
+  if (rows < 0 || width <= 0 || rows >= INT32_MAX || width > (1 << 30))
     return set_error(FG_EINVAL, "fg_log_probs: bad shape [%lld x %lld]", (long long)rows, (long long)width);
   if (!known_dtype(dtype)) return set_error(FG_EINVAL, "fg_log_probs: unknown element type %d", dtype);
   if (ld < width) return set_error(FG_EINVAL, "fg_log_probs: leading dimension smaller than the row");
@@ -496,9 +521,11 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     const T* x = static_cast<const T*>(logits);
-    // threads for a tile or two of a narrow row, so that few idle
-    if (width <= 1024) return launch_logprobs<T, 32>(a, x, s);
-    if (width <= 4096) return launch_logprobs<T, 128>(a, x, s);
+    // Threads of a block: with rows enough to fill the SMs a warp alone takes
+    // a row, without a barrier; fewer rows or a wide one get more.
+    const int64_t fill = int64_t(sm_count()) * 1024;
+    if (width <= 1024 || rows * 32 >= fill) return launch_logprobs<T, 32>(a, x, s);
+    if (width <= 4096 || rows * 128 >= fill) return launch_logprobs<T, 128>(a, x, s);
     return launch_logprobs<T, 512>(a, x, s);
   });
 }
