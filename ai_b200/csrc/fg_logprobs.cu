@@ -51,6 +51,41 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two float32 operations at once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 struct LogProbsArgs {
   int64_t rows, ld;
   int width, top;
@@ -80,54 +115,6 @@ struct RowSums {
   }
 };
 
-// One pass over each row by the blocks of a cluster (one block where there
-// are rows enough for the SMs): tiles of kItems entries a thread, the next
-// tile's loads under way while this one is summed, each thread's sums about
-// its own running maximum (moved only when a tile has a larger one). The
-// first block joins the parts through distributed shared memory.
-//
-// The alternatives: a block lists the entries that may be among its first
-// `top`, and knows a bound that `top` of them reach, so that a tile without
-// an entry above it costs a comparison and a barrier. The first bound comes
-// from the first tile: of every warp the r-th largest of its lanes' maxima,
-// r = ⌈top / warps⌉, and of these the least. Later ones are the `top`-th
-// entry whenever the list is ranked (an entry's rank is the number of
-// entries above it). A tile of which more would enter than the list holds
-// (long runs of equal or rising values) gives its best `top` one at a time.
-constexpr int kItems = 16;
-constexpr int kListSize = 512;  // entries that may wait besides the first `top`
-constexpr int kMaxSplit = 16;   // blocks of a cluster
-
-template <int THREADS>
-struct RowShared {
-  uint64_t list[kListSize + kMaxTop];
-  uint64_t best[kMaxTop];
-  uint64_t warp_key[THREADS / 32];
-  RowSums warp_sums[THREADS / 32];
-  RowSums sums;
-  uint32_t warp_bound[THREADS / 32];
-  int count;  // entries of the list
-};
-
-// Ranks the n entries of the list; the first `top` stay, in order. Returns
-// how many there are. All threads of the block.
-template <int THREADS>
-__device__ __forceinline__ int rank_list(RowShared<THREADS>& sh, int n, int top) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t mine = sh.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.list[j] > mine;
-    if (rank < top) sh.best[rank] = mine;  // entries are distinct, so ranks are
-  }
-  __syncthreads();
-  n = min(n, top);
-  for (int i = threadIdx.x; i < n; i += THREADS) sh.list[i] = sh.best[i];
-  if (threadIdx.x == 0) sh.count = n;
-  __syncthreads();
-  return n;
-}
-
 // sum += x, keeping in `lost` what the sum's rounding put in too much
 // (Kahan's summation): a long row's many small terms count beside a large one.
 __device__ __forceinline__ void add_kept(float& sum, float& lost, float x) {
@@ -156,37 +143,100 @@ __device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
   return v;
 }
 
+// One pass over each row by the warps of a block, or of a cluster of blocks
+// where there are too few rows for the SMs. A warp takes tiles of 32·kItems
+// entries, the next tile's loads under way while this one is summed; each
+// thread's sums are about its own running maximum (moved only when a tile
+// has a larger one). No warp waits for another until its row is read.
+//
+// The alternatives: every warp keeps its first `top` in order in registers,
+// one or two a lane, and a bound that `top` entries of the row reach, so that
+// a tile without an entry above it costs a comparison. An entry above it is
+// put in its place by all lanes together. The first bound comes from the
+// first tile: the top-th largest of the lanes' maxima (of half a lane's
+// entries each past 32); a tile with many entries above the bound gives
+// another one in the same way before any is taken. The warps of a block tell
+// one another their bounds in shared memory. At the end the lists are joined
+// by counting, for every entry, the entries above it.
+constexpr int kItems = 16;
+constexpr int kMany = 48;      // entries above the bound that ask for another bound first
+constexpr int kMaxSplit = 16;  // blocks of a cluster
+
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t warp_max_key(uint64_t key) {
-  const uint32_t hi = __reduce_max_sync(kFull, uint32_t(key >> 32));
-  const uint32_t lo = __reduce_max_sync(kFull, uint32_t(key >> 32) == hi ? uint32_t(key) : 0u);
-  return uint64_t(hi) << 32 | lo;
+
+// A warp's first 32·N keys in descending order: place 32·n + lane.
+template <int N>
+struct TopKeys {
+  uint64_t key[N];
+
+  __device__ __forceinline__ void insert(uint64_t x, int lane) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int above = __popc(__ballot_sync(kFull, key[n] > x));
+      if (above == 32) continue;
+      const uint64_t last = __shfl_sync(kFull, key[n], 31), up = __shfl_up_sync(kFull, key[n], 1);
+      key[n] = lane < above ? key[n] : lane == above ? x : up;
+      x = last;  // goes to the head of the next 32
+    }
+  }
+  __device__ __forceinline__ uint64_t at(int place) const {
+    uint64_t r = __shfl_sync(kFull, key[0], place & 31);
+#pragma unroll
+    for (int n = 1; n < N; ++n) {
+      const uint64_t k = __shfl_sync(kFull, key[n], place & 31);
+      if (place >= 32 * n) r = k;
+    }
+    return r;
+  }
+};
+
+template <int WARPS>
+struct RowShared {
+  uint64_t list[WARPS > 1 ? WARPS * kMaxTop : 1];
+  uint64_t best[WARPS > 1 ? kMaxTop : 1];
+  unsigned long long bound;
+  RowSums warp_sums[WARPS];
+  RowSums sums;
+  int count;  // entries of the list
+};
+
+// Ranks the n entries of the list; the first `top` go to sh.best in order.
+// All threads of the block.
+template <int WARPS>
+__device__ __forceinline__ void rank_list(RowShared<WARPS>& sh, int n, int top) {
+  for (int i = threadIdx.x; i < n; i += WARPS * 32) {
+    const uint64_t mine = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.list[j] > mine;
+    if (rank < top) sh.best[rank] = mine;  // entries are distinct, so ranks are
+  }
+  __syncthreads();
 }
 
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+// N: registers a lane for the alternatives, 0 where none are asked for.
+template <typename T, int WARPS, int N>
+__global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     logprobs_kernel(LogProbsArgs a, int split, const T* __restrict__ logits) {
   constexpr int V = 16 / int(sizeof(T));  // entries of a 16-byte group
-  constexpr int G = kItems / V;           // a thread's groups of a tile
-  constexpr int kWarps = THREADS / 32;
-  __shared__ RowShared<THREADS> sh;
+  constexpr int G = kItems / V;           // a lane's groups of a tile
+  constexpr int kTile = 32 * kItems;
+  __shared__ RowShared<WARPS> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / split;
   const int part = blockIdx.x % split;
   const T* x = logits + row * a.ld;
   // groups are those of memory: the first may begin before the row
   const int skip = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int tiles = int((int64_t(a.width) + skip + THREADS * kItems - 1) / (THREADS * kItems));
+  const int tiles = (a.width + skip + kTile - 1) / kTile;
+  const int step = WARPS * split;
   const float k = a.scale * kLog2e;
-  // column of a thread's entry i of a tile
-  auto column = [&](int tile, int i) {
-    return (tile * (THREADS * G) + (i / V) * THREADS + int(threadIdx.x)) * V - skip + i % V;
-  };
+  // column of a lane's entry i of a tile
+  auto column = [&](int tile, int i) { return tile * kTile + (i / V) * (32 * V) + lane * V - skip + i % V; };
 
   Pack<T, V> next[G];
   auto load = [&](int tile) {
-    const int first = tile * (THREADS * kItems) - skip;
-    if (first >= 0 && first + THREADS * kItems <= a.width) {
+    const int first = tile * kTile - skip;
+    if (first >= 0 && first + kTile <= a.width) {
 #pragma unroll
       for (int g = 0; g < G; ++g) next[g].load(x + column(tile, g * V));
       return;
@@ -203,6 +253,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     }
   };
 
+  int tile = part * WARPS + warp;
+  if (tile < tiles) load(tile);
   const int t = part == 0 && threadIdx.x == 0 ? a.targets[row] : -1;
   float xt = 0.f;
   if (t >= 0) {
@@ -211,22 +263,32 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     else
       atomicCAS(a.err, 0, kDevBadIndex);
   }
-  if (threadIdx.x == 0) sh.count = 0;
   RowSums sums{-INFINITY, 0.f, 0.f};
   float lost1 = 0.f, lost2 = 0.f;  // what rounding added to the sums too much
-  int n = 0;                // entries of the list
-  uint64_t bound = 0;       // `top` entries met reach this key
-  float bound_value = NAN;  // and this value; NaN: no bound yet
-  if (part < tiles) load(part);
-  __syncthreads();
-  for (int tile = part; tile < tiles; tile += split) {
+  TopKeys<N ? N : 1> list;
+#pragma unroll
+  for (int n = 0; n < (N ? N : 1); ++n) list.key[n] = 0;
+  uint64_t bound = 0;       // an entry has to be above this key
+  float bound_value = NAN;  // its value; NaN: no bound yet
+  if (N && WARPS > 1) {
+    if (threadIdx.x == 0) {
+      sh.bound = 0;
+      sh.count = 0;
+    }
+    __syncthreads();
+  }
+  for (; tile < tiles; tile += step) {
     float v[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) v[i] = next[i / V].get(i % V);
-    if (tile + split < tiles) load(tile + split);
-    float most = v[0];
+    if (tile + step < tiles) load(tile + step);
+    float half0 = max_nan(v[0], v[1]), half1 = max_nan(v[kItems / 2], v[kItems / 2 + 1]);
 #pragma unroll
-    for (int i = 1; i < kItems; ++i) most = max_nan(most, v[i]);
+    for (int i = 2; i < kItems / 2; i += 2) {
+      half0 = max3_nan(half0, v[i], v[i + 1]);
+      half1 = max3_nan(half1, v[kItems / 2 + i], v[kItems / 2 + i + 1]);
+    }
+    const float most = max_nan(half0, half1);
     const float higher = max_nan(sums.ref, most);
     if (!(higher == sums.ref)) {
       sums.s1 -= lost1;
@@ -235,117 +297,115 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       sums.move(higher, k);
     }
     const float ref = sums.ref == -INFINITY ? 0.f : sums.ref;
-    float s1 = 0.f, s2 = 0.f;
+    float2 s1 = make_float2(0.f, 0.f), s2 = s1;
+    const float2 minus = make_float2(-ref, -ref), k2 = make_float2(k, k);
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const float d = max_nan(v[i] - ref, -FLT_MAX);  // −∞ times e^−∞ = 0 would be no number
-      const float e = ex2_approx(d * k);
-      s1 += e;
-      s2 = fmaf(e, d, s2);
+    for (int i = 0; i < kItems; i += 2) {
+      float2 d = add2(make_float2(v[i], v[i + 1]), minus);
+      d = make_float2(max_nan(d.x, -FLT_MAX), max_nan(d.y, -FLT_MAX));  // −∞ times e^−∞ = 0 would be no number
+      float2 e = mul2(d, k2);
+      e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+      s1 = add2(s1, e);
+      s2 = fma2(e, d, s2);
     }
-    add_kept(sums.s1, lost1, s1);
-    add_kept(sums.s2, lost2, s2);
-    if (a.top == 0) continue;
+    add_kept(sums.s1, lost1, s1.x + s1.y);
+    add_kept(sums.s2, lost2, s2.x + s2.y);
+    if (N == 0) continue;
 
-    if (tile == part) {
-      const int r = (a.top + kWarps - 1) / kWarps;
-      // lanes without an entry of the row come last
-      uint32_t mine = column(tile, V - 1) >= 0 && column(tile, 0) < a.width ? rank_bits(most) : 0u, least = 0;
-      if (r <= 32) {
-        for (int i = 0; i < r; ++i) {
-          least = __reduce_max_sync(kFull, mine);
-          if (lane == __ffs(__ballot_sync(kFull, mine == least)) - 1) mine = 0;
-        }
-      }
-      if (lane == 0) sh.warp_bound[warp] = least;
-      __syncthreads();
-      least = __reduce_min_sync(kFull, sh.warp_bound[lane < kWarps ? lane : 0]);
-      bound = uint64_t(least) << 32;
-      if (least) bound_value = rank_value(least);
-    }
-    auto key_of = [&](int i) {
-      const int j = column(tile, i);
-      const uint64_t key = j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
-      return key > bound ? key : 0;
-    };
-    bool entered = false;
-    if (!(most < bound_value)) {
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        if (v[i] < bound_value) continue;
-        const uint64_t key = key_of(i);
-        if (key) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kListSize + kMaxTop) sh.list[at] = key;
-          entered = true;
-        }
-      }
-    }
-    if (!__syncthreads_or(entered)) continue;
-    const int before = n;
-    n = sh.count;
-    __syncthreads();
-    const bool over = n > kListSize + kMaxTop;
-    if (over) {
-      n = before;
-      uint64_t mine = 0;
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) mine = larger(mine, key_of(i));
-      for (int r = 0; r < a.top; ++r) {
-        const uint64_t w = warp_max_key(mine);
-        if (lane == 0) sh.warp_key[warp] = w;
-        __syncthreads();
-        const uint64_t first = warp_max_key(sh.warp_key[lane < kWarps ? lane : 0]);
-        if (first == 0) break;
-        if (mine == first) {
-          sh.list[n] = first;
-          mine = 0;
-#pragma unroll
-          for (int i = 0; i < kItems; ++i) {
-            const uint64_t key = key_of(i);
-            if (key < first) mine = larger(mine, key);
-          }
-        }
-        ++n;
-        __syncthreads();
-      }
-    }
-    if (over || n > kListSize || (tile + split < tiles && n >= a.top + kListSize / 8)) {
-      n = rank_list(sh, n, a.top);
-      if (n == a.top) {
-        bound = sh.list[n - 1];
+    if (WARPS > 1) {
+      const uint64_t told = *static_cast<volatile unsigned long long*>(&sh.bound);
+      if (told > bound) {
+        bound = told;
         bound_value = rank_value(uint32_t(bound >> 32));
       }
     }
+    if (!__any_sync(kFull, !(most < bound_value))) continue;
+    int above = 0;
+    if (bound) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) above += !(v[i] < bound_value);
+      above = __reduce_add_sync(kFull, above);
+    }
+    if (bound == 0 || above > kMany) {
+      // lanes without an entry of the row give no bound
+      const bool none0 = column(tile, kItems / 2 - 1) < 0 || column(tile, 0) >= a.width;
+      const bool none1 = column(tile, kItems - 1) < 0 || column(tile, kItems / 2) >= a.width;
+      uint32_t least = 0;
+      if (N == 1) {
+        uint32_t mine = none0 && none1 ? 0u : rank_bits(none1 ? half0 : none0 ? half1 : most);
+        for (int i = 0; i < a.top; ++i) {
+          least = __reduce_max_sync(kFull, mine);
+          if (lane == __ffs(__ballot_sync(kFull, mine == least)) - 1) mine = 0;
+        }
+      } else {
+        least = __reduce_min_sync(kFull, min(none0 ? 0u : rank_bits(half0), none1 ? 0u : rank_bits(half1)));
+      }
+      const uint64_t reached = uint64_t(least) << 32;
+      if (reached > bound) {
+        bound = reached;
+        bound_value = rank_value(least);
+      }
+    }
+    const uint64_t old = bound;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const bool maybe = !(v[i] < bound_value);
+      if (!__any_sync(kFull, maybe)) continue;
+      const int j = column(tile, i);
+      uint64_t key = maybe && j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
+      while (true) {
+        const unsigned who = __ballot_sync(kFull, key > bound);
+        if (!who) break;
+        const int src = __ffs(who) - 1;
+        list.insert(__shfl_sync(kFull, key, src), lane);
+        if (lane == src) key = 0;
+        const uint64_t last = list.at(a.top - 1);
+        if (last > bound) {
+          bound = last;
+          bound_value = rank_value(uint32_t(bound >> 32));
+        }
+      }
+    }
+    if (WARPS > 1 && bound > old && lane == 0) atomicMax(&sh.bound, bound);
   }
 
   const RowSums none{-INFINITY, 0.f, 0.f};
   sums.s1 -= lost1;
   sums.s2 -= lost2;
   sums = warp_join(sums, k);
-  if (kWarps > 1) {
+  if (WARPS > 1) {
     if (lane == 0) sh.warp_sums[warp] = sums;
     __syncthreads();
-    sums = warp_join(lane < kWarps ? sh.warp_sums[lane % kWarps] : none, k);
+    sums = warp_join(lane < WARPS ? sh.warp_sums[lane % WARPS] : none, k);
+    if (N) {
+      // entries that every warp's bound leaves among the first
+      const uint64_t least = sh.bound;
+#pragma unroll
+      for (int n = 0; n < (N ? N : 1); ++n)
+        if (n * 32 + lane < a.top && list.key[n] && list.key[n] >= least) sh.list[atomicAdd(&sh.count, 1)] = list.key[n];
+      __syncthreads();
+      rank_list(sh, sh.count, a.top);
+    }
   }
-  if (a.top) n = rank_list(sh, n, a.top);
   if (split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) sh.sums = sums;
     cluster.sync();
     if (part == 0) {
       sums = warp_join(lane < split ? cluster.map_shared_rank(&sh, lane % split)->sums : none, k);
-      // as many parts' lists at a time as the list has room for
-      const int batch = a.top ? kListSize / a.top : split;
-      for (int p0 = 1; a.top && p0 < split; p0 += batch) {
-        const int parts = min(batch, split - p0);
-        for (int i = threadIdx.x; i < parts * a.top; i += THREADS) {
-          const RowShared<THREADS>* other = cluster.map_shared_rank(&sh, p0 + i / a.top);
-          if (i % a.top < other->count) sh.list[atomicAdd(&sh.count, 1)] = other->list[i % a.top];
+      if (N && WARPS > 1) {
+        // a block's best are its first min(count, top)
+        const int mine = min(sh.count, a.top);
+        for (int i = threadIdx.x; i < mine; i += WARPS * 32) sh.list[i] = sh.best[i];
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = mine;
+        __syncthreads();
+        for (int i = threadIdx.x; i < (split - 1) * a.top; i += WARPS * 32) {
+          const RowShared<WARPS>* other = cluster.map_shared_rank(&sh, 1 + i / a.top);
+          if (i % a.top < other->count) sh.list[atomicAdd(&sh.count, 1)] = other->best[i % a.top];
         }
         __syncthreads();
-        n = sh.count;
-        n = rank_list(sh, n, a.top);
+        rank_list(sh, sh.count, a.top);
       }
     }
     cluster.sync();  // the parts' shared memory is read until here
@@ -359,23 +419,28 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     a.entropy[row] = empty ? 0.f : logs - a.scale * (sums.s2 / sums.s1);
     a.lse[row] = fmaf(ref, a.scale, logs);
   }
-  for (int i = threadIdx.x; i < a.top; i += THREADS) {
-    const uint64_t key = sh.list[i];
+  if (N == 0) return;
+#pragma unroll
+  for (int n = 0; n < (N ? N : 1); ++n) {
+    const int i = n * 32 + lane;
+    if (warp > 0 || i >= a.top) return;
+    const uint64_t key = WARPS > 1 ? sh.best[i] : list.key[n];
     a.top_index[row * a.top + i] = int32_t(rank_index(key));
     a.top_logprob[row * a.top + i] = empty ? -INFINITY : fmaf(rank_value(uint32_t(key >> 32)) - ref, a.scale, -logs);
   }
 }
 
-template <typename T, int THREADS>
+template <typename T, int WARPS, int N>
 int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
-  // blocks of a row: as many as fill the SMs (1024 threads each), at most one a tile
-  const int tiles = int((int64_t(a.width) + THREADS * kItems - 1) / (THREADS * kItems));
-  const int64_t room = int64_t(sm_count()) * (1024 / THREADS);
+  auto kernel = logprobs_kernel<T, WARPS, N>;
+  // blocks of a row: as many as fill the SMs (32 warps each), at most one for
+  // every WARPS tiles
+  const int64_t tiles = (int64_t(a.width) + WARPS * 32 * kItems - 1) / (WARPS * 32 * kItems);
+  const int64_t room = int64_t(sm_count()) * (32 / WARPS);
   int split = 1;
-  while (split * 2 <= std::min(kMaxSplit, tiles) && a.rows * split * 2 <= room) split *= 2;
-  auto kernel = logprobs_kernel<T, THREADS>;
+  while (WARPS == 16 && split * 2 <= std::min<int64_t>(kMaxSplit, tiles) && a.rows * split * 2 <= room) split *= 2;
   if (split == 1) {
-    kernel<<<unsigned(a.rows), THREADS, 0, s>>>(a, 1, logits);
+    kernel<<<unsigned(a.rows), WARPS * 32, 0, s>>>(a, 1, logits);
     FG_CUDA_TRY(cudaGetLastError());
     return FG_OK;
   }
@@ -386,12 +451,18 @@ int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(a.rows * split));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, split, logits));
   return FG_OK;
+}
+
+template <typename T, int WARPS>
+int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
+  if (a.top == 0) return launch_logprobs<T, WARPS, 0>(a, logits, s);
+  return a.top <= 32 ? launch_logprobs<T, WARPS, 1>(a, logits, s) : launch_logprobs<T, WARPS, 2>(a, logits, s);
 }
 
 struct LogProbsGradArgs {
@@ -521,12 +592,12 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     const T* x = static_cast<const T*>(logits);
-    // Threads of a block: with rows enough to fill the SMs a warp alone takes
+    // Warps of a row's block: with rows enough to fill the SMs a warp alone takes
     // a row, without a barrier; fewer rows or a wide one get more.
     const int64_t fill = int64_t(sm_count()) * 1024;
-    if (width <= 1024 || rows * 32 >= fill) return launch_logprobs<T, 32>(a, x, s);
-    if (width <= 4096 || rows * 128 >= fill) return launch_logprobs<T, 128>(a, x, s);
-    return launch_logprobs<T, 512>(a, x, s);
+    if (width <= 1024 || rows * 32 >= fill) return launch_logprobs<T, 1>(a, x, s);
+    if (width <= 4096 || rows * 128 >= fill) return launch_logprobs<T, 4>(a, x, s);
+    return launch_logprobs<T, 16>(a, x, s);
   });
 }
 
