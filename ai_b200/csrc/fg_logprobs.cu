@@ -151,16 +151,22 @@ __device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
 //
 // The alternatives: every warp keeps its first `top` in order in registers,
 // one or two a lane, and a bound that `top` entries of the row reach, so that
-// a tile without an entry above it costs a comparison. An entry above it is
-// put in its place by all lanes together. The first bound comes from the
-// first tile: the top-th largest of the lanes' maxima (of half a lane's
-// entries each past 32); a tile with many entries above the bound gives
-// another one in the same way before any is taken. The warps of a block tell
-// one another their bounds in shared memory. At the end the lists are joined
-// by counting, for every entry, the entries above it.
+// a tile without an entry above it costs a comparison. A tile's entries above
+// it go to shared memory; a few of them are put in their places one by one,
+// more are sorted across the lanes, 32 at a time, and merged, and either
+// gives a new bound. (Both lie outside the unrolled loop over the entries:
+// inside it they missed the instruction cache, 118 issue slots an entry.) The first
+// bound comes from the first tile: the top-th largest of the lanes' maxima
+// (of half a lane's entries each past 32); a tile with many entries above the
+// bound gives another one in the same way before any is taken. The warps of
+// a block tell one another their bounds. At the end the lists are joined by
+// counting, for every entry, the entries above it.
 constexpr int kItems = 16;
-constexpr int kMany = 48;      // entries above the bound that ask for another bound first
+constexpr int kMany = 96;      // entries of a tile above the bound that ask for another bound first
+constexpr int kFew = 3;        // entries that are put in their places one by one
 constexpr int kMaxSplit = 16;  // blocks of a cluster
+constexpr int kMaxWarps = 8;   // of a block
+static_assert(kMaxWarps <= kMaxSplit, "the list has room for either");
 
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
@@ -173,10 +179,35 @@ struct TopKeys {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int above = __popc(__ballot_sync(kFull, key[n] > x));
-      if (above == 32) continue;
       const uint64_t last = __shfl_sync(kFull, key[n], 31), up = __shfl_up_sync(kFull, key[n], 1);
       key[n] = lane < above ? key[n] : lane == above ? x : up;
-      x = last;  // goes to the head of the next 32
+      if (above < 32) x = last;  // goes to the head of the next 32
+    }
+  }
+  // One step of a bitonic network: the lanes whose `bit` is 0 keep the larger
+  // of a pair where `falling`, the others the smaller.
+  static __device__ __forceinline__ uint64_t exchange(uint64_t x, int bit, bool falling, int lane) {
+    const uint64_t other = __shfl_xor_sync(kFull, x, bit);
+    return (other > x) == (((lane & bit) == 0) == falling) ? other : x;
+  }
+  static __device__ __forceinline__ uint64_t fall(uint64_t x, int lane) {
+#pragma unroll
+    for (int bit = 16; bit > 0; bit >>= 1) x = exchange(x, bit, true, lane);
+    return x;
+  }
+  // Takes in one key a lane.
+  __device__ __forceinline__ void merge(uint64_t x, int lane) {
+    // rising over the lanes, so that the larger of each lane's two are the
+    // first 32 of both, in an order that `fall` makes descending
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+      for (int bit = size / 2; bit > 0; bit >>= 1) x = exchange(x, bit, (lane & size) != 0, lane);
+    key[N - 1] = fall(larger(key[N - 1], x), lane);
+    if (N == 2) {
+      const uint64_t rising = __shfl_sync(kFull, key[N - 1], 31 - lane);
+      key[N - 1] = fall(key[0] < rising ? key[0] : rising, lane);
+      key[0] = fall(larger(key[0], rising), lane);
     }
   }
   __device__ __forceinline__ uint64_t at(int place) const {
@@ -192,8 +223,9 @@ struct TopKeys {
 
 template <int WARPS>
 struct RowShared {
-  uint64_t list[WARPS > 1 ? WARPS * kMaxTop : 1];
+  uint64_t list[WARPS == kMaxWarps ? kMaxSplit * kMaxTop : WARPS * kMaxTop];  // of the warps, then of the blocks
   uint64_t best[WARPS > 1 ? kMaxTop : 1];
+  uint64_t found[WARPS][32 * kItems];  // a tile's entries above the bound
   unsigned long long bound;
   RowSums warp_sums[WARPS];
   RowSums sums;
@@ -282,12 +314,10 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
 #pragma unroll
     for (int i = 0; i < kItems; ++i) v[i] = next[i / V].get(i % V);
     if (tile + step < tiles) load(tile + step);
-    float half0 = max_nan(v[0], v[1]), half1 = max_nan(v[kItems / 2], v[kItems / 2 + 1]);
+    float quarter[4];
 #pragma unroll
-    for (int i = 2; i < kItems / 2; i += 2) {
-      half0 = max3_nan(half0, v[i], v[i + 1]);
-      half1 = max3_nan(half1, v[kItems / 2 + i], v[kItems / 2 + i + 1]);
-    }
+    for (int q = 0; q < 4; ++q) quarter[q] = max3_nan(max_nan(v[4 * q], v[4 * q + 1]), v[4 * q + 2], v[4 * q + 3]);
+    const float half0 = max_nan(quarter[0], quarter[1]), half1 = max_nan(quarter[2], quarter[3]);
     const float most = max_nan(half0, half1);
     const float higher = max_nan(sums.ref, most);
     if (!(higher == sums.ref)) {
@@ -344,29 +374,41 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
       if (reached > bound) {
         bound = reached;
         bound_value = rank_value(least);
+        if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
       }
     }
-    const uint64_t old = bound;
+    uint64_t* found = sh.found[warp];
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const bool maybe = !(v[i] < bound_value);
-      if (!__any_sync(kFull, maybe)) continue;
-      const int j = column(tile, i);
-      uint64_t key = maybe && j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
-      while (true) {
+    for (int q = 0; q < 4; ++q) {
+      if (!__any_sync(kFull, !(quarter[q] < bound_value))) continue;
+#pragma unroll
+      for (int i = 4 * q; i < 4 * q + 4; ++i) {
+        const bool maybe = !(v[i] < bound_value);
+        if (!__any_sync(kFull, maybe)) continue;
+        const int j = column(tile, i);
+        const uint64_t key = maybe && j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
         const unsigned who = __ballot_sync(kFull, key > bound);
-        if (!who) break;
-        const int src = __ffs(who) - 1;
-        list.insert(__shfl_sync(kFull, key, src), lane);
-        if (lane == src) key = 0;
-        const uint64_t last = list.at(a.top - 1);
-        if (last > bound) {
-          bound = last;
-          bound_value = rank_value(uint32_t(bound >> 32));
-        }
+        if (key > bound) found[n + __popc(who & ((1u << lane) - 1))] = key;
+        n += __popc(who);
       }
     }
-    if (WARPS > 1 && bound > old && lane == 0) atomicMax(&sh.bound, bound);
+    if (n == 0) continue;
+    __syncwarp();
+    if (n <= kFew) {
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) list.insert(found[i], lane);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < n; i += 32) list.merge(i + lane < n ? found[i + lane] : 0, lane);
+    }
+    __syncwarp();
+    const uint64_t last = list.at(a.top - 1);
+    if (last > bound) {
+      bound = last;
+      bound_value = rank_value(uint32_t(bound >> 32));
+      if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
+    }
   }
 
   const RowSums none{-INFINITY, 0.f, 0.f};
@@ -438,7 +480,7 @@ int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
   const int64_t tiles = (int64_t(a.width) + WARPS * 32 * kItems - 1) / (WARPS * 32 * kItems);
   const int64_t room = int64_t(sm_count()) * (32 / WARPS);
   int split = 1;
-  while (WARPS == 16 && split * 2 <= std::min<int64_t>(kMaxSplit, tiles) && a.rows * split * 2 <= room) split *= 2;
+  while (WARPS == kMaxWarps && split * 2 <= std::min<int64_t>(kMaxSplit, tiles) && a.rows * split * 2 <= room) split *= 2;
   if (split == 1) {
     kernel<<<unsigned(a.rows), WARPS * 32, 0, s>>>(a, 1, logits);
     FG_CUDA_TRY(cudaGetLastError());
@@ -596,8 +638,8 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
     // a row, without a barrier; fewer rows or a wide one get more.
     const int64_t fill = int64_t(sm_count()) * 1024;
     if (width <= 1024 || rows * 32 >= fill) return launch_logprobs<T, 1>(a, x, s);
-    if (width <= 4096 || rows * 128 >= fill) return launch_logprobs<T, 4>(a, x, s);
-    return launch_logprobs<T, 16>(a, x, s);
+    if (width <= 4096) return launch_logprobs<T, 4>(a, x, s);
+    return launch_logprobs<T, kMaxWarps>(a, x, s);
   });
 }
 
