@@ -162,7 +162,7 @@ __device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
 // a block tell one another their bounds. At the end the lists are joined by
 // counting, for every entry, the entries above it.
 constexpr int kItems = 16;
-constexpr int kMany = 96;      // entries of a tile above the bound that ask for another bound first
+constexpr int kMany = 24;      // lanes with entries above the bound that ask for another bound first
 constexpr int kFew = 3;        // entries that are put in their places one by one
 constexpr int kMaxSplit = 16;  // blocks of a cluster
 constexpr int kMaxWarps = 8;   // of a block
@@ -225,7 +225,7 @@ template <int WARPS>
 struct RowShared {
   uint64_t list[WARPS == kMaxWarps ? kMaxSplit * kMaxTop : WARPS * kMaxTop];  // of the warps, then of the blocks
   uint64_t best[WARPS > 1 ? kMaxTop : 1];
-  uint64_t found[WARPS][32 * kItems];  // a tile's entries above the bound
+  uint2 found[WARPS][32 * kItems];  // a tile's entries that may be above the bound: value and column
   unsigned long long bound;
   RowSums warp_sums[WARPS];
   RowSums sums;
@@ -300,8 +300,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   TopKeys<N ? N : 1> list;
 #pragma unroll
   for (int n = 0; n < (N ? N : 1); ++n) list.key[n] = 0;
-  uint64_t bound = 0;       // an entry has to be above this key
-  float bound_value = NAN;  // its value; NaN: no bound yet
+  uint64_t bound = 0;  // an entry has to be above this key; 0: no bound yet
   if (N && WARPS > 1) {
     if (threadIdx.x == 0) {
       sh.bound = 0;
@@ -342,71 +341,66 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     add_kept(sums.s2, lost2, s2.x + s2.y);
     if (N == 0) continue;
 
-    if (WARPS > 1) {
-      const uint64_t told = *static_cast<volatile unsigned long long*>(&sh.bound);
-      if (told > bound) {
-        bound = told;
-        bound_value = rank_value(uint32_t(bound >> 32));
-      }
-    }
-    if (!__any_sync(kFull, !(most < bound_value))) continue;
-    int above = 0;
-    if (bound) {
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) above += !(v[i] < bound_value);
-      above = __reduce_add_sync(kFull, above);
-    }
-    if (bound == 0 || above > kMany) {
+    if (WARPS > 1) bound = larger(bound, *static_cast<volatile unsigned long long*>(&sh.bound));
+    // the least value that may be above the bound: its own value is not when
+    // its column comes before the tile's
+    auto least_value = [&]() {
+      return bound ? rank_value(uint32_t(bound >> 32) + (int64_t(rank_index(bound)) < column(tile, 0) - lane * V)) : NAN;
+    };
+    float least = least_value();
+    const unsigned lanes = __ballot_sync(kFull, !(most < least));
+    if (lanes == 0) continue;
+    if (bound == 0 || __popc(lanes) > kMany) {
       // lanes without an entry of the row give no bound
       const bool none0 = column(tile, kItems / 2 - 1) < 0 || column(tile, 0) >= a.width;
       const bool none1 = column(tile, kItems - 1) < 0 || column(tile, kItems / 2) >= a.width;
-      uint32_t least = 0;
+      uint32_t reached = 0;
       if (N == 1) {
         uint32_t mine = none0 && none1 ? 0u : rank_bits(none1 ? half0 : none0 ? half1 : most);
         for (int i = 0; i < a.top; ++i) {
-          least = __reduce_max_sync(kFull, mine);
-          if (lane == __ffs(__ballot_sync(kFull, mine == least)) - 1) mine = 0;
+          reached = __reduce_max_sync(kFull, mine);
+          if (lane == __ffs(__ballot_sync(kFull, mine == reached)) - 1) mine = 0;
         }
       } else {
-        least = __reduce_min_sync(kFull, min(none0 ? 0u : rank_bits(half0), none1 ? 0u : rank_bits(half1)));
+        reached = __reduce_min_sync(kFull, min(none0 ? 0u : rank_bits(half0), none1 ? 0u : rank_bits(half1)));
       }
-      const uint64_t reached = uint64_t(least) << 32;
-      if (reached > bound) {
-        bound = reached;
-        bound_value = rank_value(least);
+      if (uint64_t(reached) << 32 > bound) {
+        bound = uint64_t(reached) << 32;
         if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
+        least = least_value();
       }
     }
-    uint64_t* found = sh.found[warp];
+    uint2* found = sh.found[warp];
     int n = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (!__any_sync(kFull, !(quarter[q] < bound_value))) continue;
+      if (!__any_sync(kFull, !(quarter[q] < least))) continue;
 #pragma unroll
       for (int i = 4 * q; i < 4 * q + 4; ++i) {
-        const bool maybe = !(v[i] < bound_value);
-        if (!__any_sync(kFull, maybe)) continue;
-        const int j = column(tile, i);
-        const uint64_t key = maybe && j >= 0 && j < a.width ? rank_key(v[i], uint32_t(j)) : 0;
-        const unsigned who = __ballot_sync(kFull, key > bound);
-        if (key > bound) found[n + __popc(who & ((1u << lane) - 1))] = key;
+        const bool maybe = !(v[i] < least);
+        const unsigned who = __ballot_sync(kFull, maybe);
+        if (!who) continue;
+        if (maybe) found[n + __popc(who & ((1u << lane) - 1))] = make_uint2(__float_as_uint(v[i]), column(tile, i));
         n += __popc(who);
       }
     }
     if (n == 0) continue;
     __syncwarp();
+    auto key_of = [&](int i) {
+      const uint2 f = found[i];
+      return int(f.y) >= 0 && int(f.y) < a.width ? rank_key(__uint_as_float(f.x), f.y) : uint64_t(0);
+    };
     if (n <= kFew) {
 #pragma unroll 1
-      for (int i = 0; i < n; ++i) list.insert(found[i], lane);
+      for (int i = 0; i < n; ++i) list.insert(key_of(i), lane);
     } else {
 #pragma unroll 1
-      for (int i = 0; i < n; i += 32) list.merge(i + lane < n ? found[i + lane] : 0, lane);
+      for (int i = 0; i < n; i += 32) list.merge(i + lane < n ? key_of(i + lane) : 0, lane);
     }
     __syncwarp();
     const uint64_t last = list.at(a.top - 1);
     if (last > bound) {
       bound = last;
-      bound_value = rank_value(uint32_t(bound >> 32));
       if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
     }
   }
@@ -421,10 +415,10 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     sums = warp_join(lane < WARPS ? sh.warp_sums[lane % WARPS] : none, k);
     if (N) {
       // entries that every warp's bound leaves among the first
-      const uint64_t least = sh.bound;
+      const uint64_t reached = sh.bound;
 #pragma unroll
       for (int n = 0; n < (N ? N : 1); ++n)
-        if (n * 32 + lane < a.top && list.key[n] && list.key[n] >= least) sh.list[atomicAdd(&sh.count, 1)] = list.key[n];
+        if (n * 32 + lane < a.top && list.key[n] && list.key[n] >= reached) sh.list[atomicAdd(&sh.count, 1)] = list.key[n];
       __syncthreads();
       rank_list(sh, sh.count, a.top);
     }
