@@ -11,6 +11,8 @@
 // registers and joins the runs that cross chunks in a second kernel. Sums
 // are in 32 bits in an order that depends on the ids alone, so a repeated
 // call gives the same bits; a sum is rounded once, when its row is written.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "fg_kernels.cuh"
@@ -20,6 +22,8 @@
 namespace fg {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -258,6 +262,253 @@ __global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* coun
   if (i < n && i >= *count) row_ids[i] = -1;
 }
 
+// -------------------------------------------------- sort within a cluster
+// The same sort without a trip to memory between its passes: a cluster of up
+// to 16 blocks holds all tokens in its shared memory, kItems a thread. Per
+// pass every warp ranks its tokens among those of their digit (match_any,
+// 32 at a time), the blocks exchange their digits' totals and every token
+// goes to its place in the block that holds it, through distributed shared
+// memory. 131072 tokens of 19-bit keys take two passes; through memory, in
+// nine launches, 152 us (measured), most of it latency.
+constexpr int kGroupThreads = 1024;
+constexpr int kGroupWarps = kGroupThreads / 32;
+constexpr int kMaxRadix = 1 << kMaxDigit;
+constexpr int kMinDigit = 6;  // a word of two counters for every lane of a warp
+constexpr int kMaxBlocks = 16;
+constexpr int kMaxGroupItems = 16;
+
+struct GroupArgs {
+  const int32_t* ids;
+  int n;
+  int64_t vocab;
+  int padding, passes, digit;
+  uint32_t* keys;
+  uint32_t* pos;
+  uint32_t* place;  // with row_ids and count: the rows met; null: not asked for
+  int32_t* row_ids;
+  int32_t* count;
+  int* err;
+};
+
+template <int ITEMS>
+struct GroupShared {
+  uint2 item[kGroupThreads * ITEMS];                  // (key, position) in this block's part of the order
+  uint32_t counter[kGroupWarps][kMaxRadix / 2];       // two 16-bit counters a word
+  uint32_t offset[kGroupThreads];                     // of a group of warps, two 16-bit counters a word
+  uint32_t total[kMaxRadix], base[kMaxRadix];
+  uint32_t warp_sum[kGroupWarps];
+  uint32_t heads[kGroupWarps * ITEMS];
+  uint32_t block_heads;
+};
+
+// Exclusive sum over the block's threads of v; the total in *all.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sum, uint32_t* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(kFull, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) warp_sum[warp] = s;
+  __syncthreads();
+  uint32_t w = warp_sum[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(kFull, w, o);
+    if (lane >= o) w += u;
+  }
+  *all = __shfl_sync(kFull, w, 31);
+  const uint32_t before = __shfl_sync(kFull, w, (warp + 31) & 31);
+  __syncthreads();
+  return s - v + (warp ? before : 0);
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
+  constexpr int kPart = kGroupThreads * ITEMS;  // a block's tokens
+  extern __shared__ __align__(16) unsigned char smem[];
+  GroupShared<ITEMS>& sh = *reinterpret_cast<GroupShared<ITEMS>*>(smem);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = gridDim.x, block = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int radix = 1 << a.digit, words = radix / 2;
+  // warps whose counters one thread adds up; a thread's word of them
+  const int groups = kGroupThreads / words, group_warps = kGroupWarps / groups;
+
+  uint2 mine[ITEMS];  // consecutive tokens of a warp, 32 a round
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = block * kPart + (warp * ITEMS + k) * 32 + lane;
+    // places past the last token sort behind every key
+    mine[k] = make_uint2(i < a.n ? token_key(a.ids[i], a.vocab, a.padding, a.err) : 0xffffffffu, i);
+  }
+  for (int p = 0; p < a.passes; ++p) {
+    const int shift = p * a.digit;
+    for (int i = tid; i < kGroupWarps * words; i += kGroupThreads) sh.counter[i / words][i % words] = 0;
+    __syncthreads();
+    uint16_t* count = reinterpret_cast<uint16_t*>(sh.counter[warp]);
+    uint32_t rank[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const uint32_t d = (mine[k].x >> shift) & (radix - 1);
+      const unsigned same = __match_any_sync(kFull, d);
+      const uint32_t before = __popc(same & ((1u << lane) - 1)), seen = count[d];
+      rank[k] = seen + before;
+      __syncwarp();
+      if (before == 0) count[d] = uint16_t(seen + __popc(same));
+      __syncwarp();
+    }
+    __syncthreads();
+    {
+      const int word = tid % words, group = tid / words;
+      uint32_t run = 0;  // both halves at once: a block has fewer than 2^16 tokens
+      for (int w = group * group_warps; w < (group + 1) * group_warps; ++w) {
+        const uint32_t c = sh.counter[w][word];
+        sh.counter[w][word] = run;
+        run += c;
+      }
+      sh.offset[group * words + word] = run;
+    }
+    __syncthreads();
+    if (tid < words) {
+      uint32_t run = 0;
+      for (int g = 0; g < groups; ++g) {
+        const uint32_t c = sh.offset[g * words + tid];
+        sh.offset[g * words + tid] = run;
+        run += c;
+      }
+      sh.total[2 * tid] = run & 0xffffu;
+      sh.total[2 * tid + 1] = run >> 16;
+    }
+    cluster.sync();
+    uint32_t all = 0, before = 0;
+    if (tid < radix) {
+      for (int b = 0; b < blocks; ++b) {
+        const uint32_t c = cluster.map_shared_rank(&sh, b)->total[tid];
+        all += c;
+        if (b < block) before += c;
+      }
+    }
+    uint32_t sum;
+    const uint32_t first = block_scan(all, sh.warp_sum, &sum);
+    if (tid < radix) sh.base[tid] = first + before;
+    __syncthreads();
+    const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset) + (warp / group_warps) * radix;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const uint32_t d = (mine[k].x >> shift) & (radix - 1);
+      const uint32_t to = sh.base[d] + offset[d] + count[d] + rank[k];
+      cluster.map_shared_rank(&sh, to / kPart)->item[to % kPart] = mine[k];
+    }
+    cluster.sync();
+    if (p + 1 < a.passes) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) mine[k] = sh.item[(warp * ITEMS + k) * 32 + lane];
+    }
+  }
+  // the tokens in order, and where the rows begin
+  const uint32_t left = block > 0 ? cluster.map_shared_rank(&sh, block - 1)->item[kPart - 1].x : 0xffffffffu;
+  unsigned heads[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int at = k * kGroupThreads + tid, i = block * kPart + at;
+    const uint2 it = sh.item[at];
+    const uint32_t prev = at > 0 ? sh.item[at - 1].x : left;
+    if (i < a.n) {
+      a.keys[i] = it.x;
+      a.pos[i] = it.y;
+    }
+    heads[k] = __ballot_sync(kFull, it.x < a.vocab && (i == 0 || prev != it.x));
+    if (lane == 0) sh.heads[k * kGroupWarps + warp] = __popc(heads[k]);
+  }
+  if (!a.place) {
+    cluster.sync();  // a block's last token is read until here
+    return;
+  }
+  __syncthreads();
+  // heads before each warp's round, in the block
+  const bool mine_counts = tid < kGroupWarps * ITEMS;
+  uint32_t block_heads;
+  const uint32_t before_me = block_scan(mine_counts ? sh.heads[tid % (kGroupWarps * ITEMS)] : 0, sh.warp_sum, &block_heads);
+  if (mine_counts) sh.heads[tid] = before_me;
+  if (tid == 0) sh.block_heads = block_heads;
+  cluster.sync();
+  uint32_t before = 0, total = 0;
+  for (int b = 0; b < blocks; ++b) {
+    const uint32_t c = cluster.map_shared_rank(&sh, b)->block_heads;
+    total += c;
+    if (b < block) before += c;
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int at = k * kGroupThreads + tid, i = block * kPart + at;
+    if (i >= a.n) continue;
+    const uint32_t key = sh.item[at].x;
+    const uint32_t upto = before + sh.heads[k * kGroupWarps + warp] + __popc(heads[k] & (kFull >> (31 - lane)));
+    if (key < a.vocab) a.place[i] = upto - 1;
+    if (heads[k] >> lane & 1) a.row_ids[upto - 1] = int32_t(key);
+    if (uint32_t(i) >= total) a.row_ids[i] = -1;
+  }
+  if (block == 0 && tid == 0) *a.count = int32_t(total);
+  cluster.sync();  // the blocks' counts are read until here
+}
+
+template <int ITEMS>
+int launch_group(const GroupArgs& a, int blocks, cudaStream_t s) {
+  auto kernel = group_kernel<ITEMS>;
+  FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GroupShared<ITEMS>))));
+  if (blocks > 8) FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(blocks);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(kGroupThreads);
+  cfg.dynamicSmemBytes = sizeof(GroupShared<ITEMS>);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  return FG_OK;
+}
+
+// Most tokens that a cluster sorts.
+constexpr int64_t kMaxGroup = int64_t(kMaxBlocks) * kGroupThreads * kMaxGroupItems;
+
+int group_tokens(const GroupArgs& a, cudaStream_t s) {
+  // as many blocks as the tokens fill, then more tokens a thread
+  int blocks = 1, items = 1;
+  while (blocks < kMaxBlocks && blocks * kGroupThreads < a.n) blocks *= 2;
+  while (int64_t(blocks) * kGroupThreads * items < a.n) items *= 2;
+  switch (items) {
+    case 1: return launch_group<1>(a, blocks, s);
+    case 2: return launch_group<2>(a, blocks, s);
+    case 4: return launch_group<4>(a, blocks, s);
+    case 8: return launch_group<8>(a, blocks, s);
+    default: return launch_group<16>(a, blocks, s);
+  }
+}
+
+// The first sorted token whose key is at least k, looked for by a warp: each
+// step probes 32 places.
+__device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, int64_t k, int lane) {
+  int64_t lo = 0, hi = n;  // it lies in [lo, hi]
+  while (hi > lo) {
+    const int64_t step = (hi - lo + 31) / 32, p = lo + lane * step;
+    const int c = __popc(__ballot_sync(kFull, p < hi && keys[p] < k));
+    if (c == 0) {
+      hi = lo;
+    } else {
+      const int64_t last = lo + (c - 1) * step;
+      hi = last + step < hi ? last + step : hi;
+      lo = last + 1;
+    }
+  }
+  return lo;
+}
+
 // ------------------------------------------------------------------ sums
 // A warp sums one chunk of sorted tokens over 32·VEC columns, with kAhead
 // rows in flight. A run of one id that lies within the chunk is written as
@@ -353,32 +604,88 @@ __global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(SumArgs a, const TY
 }
 
 // The runs that cross chunks: the chunk in which one begins adds the heads
-// of the chunks after it, in their order, and writes the row.
+// of the chunks after it, in their order, and writes the row. A warp joins a
+// run of a few chunks; a long one (a frequent token) is shared by the block's
+// warps, which take equal consecutive parts of it. A block's warps have
+// different chunks of the same columns, so the columns of a long run meet in
+// different blocks.
+constexpr int kLongRun = 16;  // chunks after the first
+
 template <typename TG, int VEC>
 __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* grad) {
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
-  int64_t chunk = unit / a.slices;
-  const int col = (int(unit % a.slices) * 32 + lane) * VEC;
-  const int64_t i0 = chunk * kChunk, end = i0 + kChunk;
-  if (end >= a.n) return;
-  const uint32_t key = a.keys[end - 1];
-  if (key >= a.vocab || a.keys[end] != key) return;  // no run goes on
-  if (a.keys[i0] == key && i0 > 0 && a.keys[i0 - 1] == key) return;  // it began earlier
-  if (col >= a.dim) return;
+  __shared__ int long_run[kSumWarps];
+  __shared__ float part[kSumWarps][32 * VEC];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t chunks = (a.n + kChunk - 1) / kChunk;
+  const int64_t blocks = (chunks + kSumWarps - 1) / kSumWarps;  // of a slice
+  const int64_t chunk0 = blockIdx.x % blocks * kSumWarps;
+  const int col = (int(blockIdx.x / blocks) * 32 + lane) * VEC;
+  const bool in = col < a.dim;
+  // sum of heads [c, c + count) in order, eight in flight
+  auto add_heads = [&](float (&acc)[VEC], int64_t c, int count) {
+    if (!in) return;
+    for (int i = 0; i < count; i += kAhead) {
+      Pack<float, VEC> h[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u < count) h[u].load(a.head + (c + i + u) * a.dim + col);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u < count)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += h[u].get(j);
+    }
+  };
+  auto finish = [&](const float (&acc)[VEC], int64_t chunk) {
+    const int64_t last = chunk * kChunk + kChunk - 1;
+    const int64_t row = a.place ? a.place[last] : a.keys[last];
+    if (in) write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
+  };
+
+  const int64_t chunk = chunk0 + warp, i0 = chunk * kChunk, end = i0 + kChunk;
+  int run = 0;  // chunks after this one that the run which leaves it covers
+  if (end < a.n) {
+    const uint32_t key = a.keys[end - 1];
+    const bool began = a.keys[i0] != key || i0 == 0 || a.keys[i0 - 1] != key;
+    if (key < a.vocab && a.keys[end] == key && began) {
+      // chunks that begin with the key: the last is the run's last
+      const int64_t next = first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane);
+      run = int((next + kChunk - 1) / kChunk);
+    }
+  }
   float acc[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = a.tail[chunk * a.dim + col + i];
-  const int64_t row = a.place ? a.place[end - 1] : key;
-  while (true) {
-    ++chunk;
-    const float* h = a.head + chunk * a.dim + col;
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+  if (run > 0 && run <= kLongRun) {
+    if (in)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] += h[i];
-    const int64_t next = (chunk + 1) * kChunk;
-    if (next >= a.n || a.keys[next] != key || a.keys[next - 1] != key) break;
+      for (int j = 0; j < VEC; ++j) acc[j] = a.tail[chunk * a.dim + col + j];
+    add_heads(acc, chunk + 1, run);
+    finish(acc, chunk);
   }
-  write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
+  if (lane == 0) long_run[warp] = run > kLongRun ? run : 0;
+  __syncthreads();
+  for (int w = 0; w < kSumWarps; ++w) {
+    const int count = long_run[w];
+    if (count == 0) continue;
+    const int share = (count + kSumWarps - 1) / kSumWarps, first = warp * share;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    add_heads(acc, chunk0 + w + 1 + first, max(0, min(share, count - first)));
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) part[warp][lane * VEC + j] = acc[j];
+    __syncthreads();
+    if (warp == w) {
+      if (in)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = a.tail[chunk * a.dim + col + j];
+      for (int p = 0; p < kSumWarps; ++p)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += part[p][lane * VEC + j];
+      finish(acc, chunk);
+    }
+    __syncthreads();
+  }
 }
 
 // Zeros in the rows of the dense gradient that no token met (count null;
@@ -393,27 +700,17 @@ __global__ void __launch_bounds__(kSumWarps * 32) zero_rows_kernel(const uint32_
   if (r0 >= rows) return;
   unsigned met = 0;
   if (!count) {
-    // first sorted token with a key >= r0: each step probes 32 places
-    int64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
-    while (hi > lo) {
-      const int64_t step = (hi - lo + 31) / 32;
-      const int64_t p = lo + lane * step;
-      const bool below = p < hi && keys[p] < r0;
-      const int c = __popc(__ballot_sync(kFull, below));
-      if (c == 0) {
-        hi = lo;
-      } else {
-        const int64_t last = lo + (c - 1) * step;
-        hi = last + step < hi ? last + step : hi;
-        lo = last + 1;
-      }
+    // the sorted tokens of the 32 rows are [lo, hi); each lane looks its row up
+    const int64_t lo = first_token(keys, n, r0, lane), hi = first_token(keys, n, r0 + 32, lane);
+    int64_t l = lo, h = hi;
+    while (l < h) {
+      const int64_t mid = (l + h) / 2;
+      if (keys[mid] < r0 + lane)
+        l = mid + 1;
+      else
+        h = mid;
     }
-    for (int64_t i = lo; i < n; i += 32) {
-      const uint32_t k = i + lane < n ? keys[i + lane] : 0xffffffffu;
-      const bool mine = k < r0 + 32 && k >= r0;
-      met |= __reduce_or_sync(kFull, mine ? 1u << (k - r0) : 0u);
-      if (!__all_sync(kFull, mine)) break;
-    }
+    met = __ballot_sync(kFull, l < hi && keys[l] == r0 + lane);
   } else {
     const int64_t c = *count;
     met = c >= r0 + 32 ? kFull : c > r0 ? (1u << (c - r0)) - 1 : 0;
@@ -471,7 +768,12 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   SumArgs a{};
   a.head = static_cast<float*>(take(part));
   a.tail = static_cast<float*>(take(part));
-  if (n > 0) {
+  const bool grouped_here = n <= kMaxGroup;
+  if (n > 0 && grouped_here) {
+    GroupArgs g{ids, int(n), vocab, padding, passes, std::max(digit, kMinDigit), key[0], pos[0], compact ? place : nullptr,
+                row_ids, count, err};
+    FG_TRY(group_tokens(g, s));
+  } else if (n > 0) {
     for (int p = 0; p < passes; ++p) {
       const uint32_t* k = p ? key[(p + 1) & 1] : nullptr;
       sort_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, n, vocab, padding, p * digit, digit, counts, err);
@@ -480,8 +782,8 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
                                                                p * digit, digit, counts, key[p & 1], pos[p & 1], err);
     }
   }
-  a.keys = key[(passes - 1) & 1];
-  a.pos = pos[(passes - 1) & 1];
+  a.keys = key[grouped_here ? 0 : (passes - 1) & 1];
+  a.pos = pos[grouped_here ? 0 : (passes - 1) & 1];
   a.n = n;
   a.vocab = vocab;
   a.dim = int(dim);
@@ -489,12 +791,12 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.ldg = ldg;
   a.scale = scale;
   a.accumulate = accumulate;
-  if (compact) {
+  if (compact) a.place = place;
+  if (compact && !grouped_here) {
     heads_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts);
     scan_kernel<<<1, kScanThreads, 0, s>>>(counts, tiles, count);
     heads_place_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts, place, row_ids);
     rest_ids_kernel<<<unsigned(blocks_of(n, 256)), 256, 0, s>>>(row_ids, n, count);
-    a.place = place;
   }
   FG_CUDA_TRY(cudaGetLastError());
   const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
@@ -524,10 +826,11 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
       FG_CUDA_TRY(cudaGetLastError());
       return FG_OK;
     }));
+    const unsigned join_blocks = unsigned(blocks_of(chunks, kSumWarps) * a.slices);
     if (wide)
-      join_kernel<TG, 4><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, g);
+      join_kernel<TG, 4><<<join_blocks, kSumWarps * 32, 0, s>>>(a, g);
     else
-      join_kernel<TG, 1><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, g);
+      join_kernel<TG, 1><<<join_blocks, kSumWarps * 32, 0, s>>>(a, g);
     FG_CUDA_TRY(cudaGetLastError());
     return FG_OK;
   });
