@@ -263,28 +263,36 @@ __global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* coun
 }
 
 // -------------------------------------------------- sort within a cluster
-// The same sort without a trip to memory between its passes: a cluster of up
-// to 16 blocks holds all tokens in its shared memory, kItems a thread. Per
-// pass every warp ranks its tokens among those of their digit (match_any,
-// 32 at a time), the blocks exchange their digits' totals and every token
-// goes to its place in the block that holds it, through distributed shared
-// memory. 131072 tokens of 19-bit keys take two passes; through memory, in
-// nine launches, 152 us (measured), most of it latency.
+// The same sort in one launch: the tokens lie in the registers of a cluster
+// of up to 16 blocks, ITEMS a thread, and the blocks wait for one another at
+// the cluster's barrier only. Per pass of kMaxDigit bits every warp ranks its
+// tokens among those of their digit, 32 at a time; a block orders its tokens
+// by digit in shared memory, so that neighbouring lanes write neighbouring
+// places; and with all blocks' digit totals every token goes to its place.
+// Totals and tokens are exchanged through L2. Measured on 131072 tokens of
+// 19 bits: distributed shared memory moved 5 to 7 bytes a cycle and SM, 14200
+// cycles a pass for the tokens and 9600 for the totals; lanes of one digit
+// found by match_any took 2300 cycles a round (a step for every distinct
+// digit), by a vote a bit 950.
 constexpr int kGroupThreads = 1024;
 constexpr int kGroupWarps = kGroupThreads / 32;
-constexpr int kMaxRadix = 1 << kMaxDigit;
-constexpr int kMinDigit = 6;  // a word of two counters for every lane of a warp
+constexpr int kRadix = 1 << kMaxDigit;
+constexpr int kWords = kRadix / 2;                    // two 16-bit counters each
+constexpr int kHalf = kGroupThreads / kWords;         // threads that share a word's sum over the warps
+constexpr int kHalfWarps = kGroupWarps / kHalf;
 constexpr int kMaxBlocks = 16;
+static_assert(kRadix == kGroupThreads, "a thread for every digit");
 constexpr int kMaxGroupItems = 16;
 
 struct GroupArgs {
   const int32_t* ids;
   int n;
   int64_t vocab;
-  int padding, passes, digit;
-  uint32_t* keys;
-  uint32_t* pos;
-  uint32_t* place;  // with row_ids and count: the rows met; null: not asked for
+  int padding, passes;
+  uint32_t* totals;  // [kMaxBlocks, kRadix] and kMaxBlocks more
+  uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
+  uint32_t* pos[2];
+  uint32_t* place;   // with row_ids and count: the rows met; null: not asked for
   int32_t* row_ids;
   int32_t* count;
   int* err;
@@ -292,13 +300,14 @@ struct GroupArgs {
 
 template <int ITEMS>
 struct GroupShared {
-  uint2 item[kGroupThreads * ITEMS];                  // (key, position) in this block's part of the order
-  uint32_t counter[kGroupWarps][kMaxRadix / 2];       // two 16-bit counters a word
-  uint32_t offset[kGroupThreads];                     // of a group of warps, two 16-bit counters a word
-  uint32_t total[kMaxRadix], base[kMaxRadix];
+  union {
+    uint32_t counter[kGroupWarps][kWords];  // of every warp's tokens
+    uint2 local[kGroupThreads * ITEMS];     // then the block's tokens ordered by digit
+  };
+  uint32_t offset[kHalf][kWords];
+  uint32_t base[kRadix], start[kRadix];
   uint32_t warp_sum[kGroupWarps];
   uint32_t heads[kGroupWarps * ITEMS];
-  uint32_t block_heads;
 };
 
 // Exclusive sum over the block's threads of v; the total in *all.
@@ -332,27 +341,43 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = gridDim.x, block = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int radix = 1 << a.digit, words = radix / 2;
-  // warps whose counters one thread adds up; a thread's word of them
-  const int groups = kGroupThreads / words, group_warps = kGroupWarps / groups;
-
-  uint2 mine[ITEMS];  // consecutive tokens of a warp, 32 a round
+  uint2 mine[ITEMS];  // (key, position) of consecutive tokens of a warp, 32 a round
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int i = block * kPart + (warp * ITEMS + k) * 32 + lane;
-    // places past the last token sort behind every key
-    mine[k] = make_uint2(i < a.n ? token_key(a.ids[i], a.vocab, a.padding, a.err) : 0xffffffffu, i);
+    mine[k] = make_uint2(i < a.n ? uint32_t(a.ids[i]) : 0u, i);
   }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)  // places past the last token sort behind every key
+    mine[k].x = int(mine[k].y) < a.n ? token_key(int(mine[k].x), a.vocab, a.padding, a.err) : 0xffffffffu;
   for (int p = 0; p < a.passes; ++p) {
-    const int shift = p * a.digit;
-    for (int i = tid; i < kGroupWarps * words; i += kGroupThreads) sh.counter[i / words][i % words] = 0;
+    const int shift = p * kMaxDigit;
+    uint32_t* key_to = a.key[(a.passes - 1 - p) & 1];
+    uint32_t* pos_to = a.pos[(a.passes - 1 - p) & 1];
+    if (p > 0) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int i = block * kPart + (warp * ITEMS + k) * 32 + lane;
+        mine[k] = i < a.n ? make_uint2(__ldcg(a.key[(a.passes - p) & 1] + i), __ldcg(a.pos[(a.passes - p) & 1] + i))
+                          : make_uint2(0xffffffffu, i);
+      }
+    }
+    uint4* zero = reinterpret_cast<uint4*>(&sh.counter[0][0]);
+#pragma unroll
+    for (int i = 0; i < kGroupWarps * kWords / 4; i += kGroupThreads) zero[i + tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     uint16_t* count = reinterpret_cast<uint16_t*>(sh.counter[warp]);
     uint32_t rank[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & (radix - 1);
-      const unsigned same = __match_any_sync(kFull, d);
+      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1);
+      unsigned same = kFull;
+#pragma unroll
+      for (int b = 0; b < kMaxDigit; ++b) {
+        const bool set = d >> b & 1;
+        const unsigned vote = __ballot_sync(kFull, set);
+        same &= set ? vote : ~vote;
+      }
       const uint32_t before = __popc(same & ((1u << lane) - 1)), seen = count[d];
       rank[k] = seen + before;
       __syncwarp();
@@ -361,97 +386,106 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     }
     __syncthreads();
     {
-      const int word = tid % words, group = tid / words;
-      uint32_t run = 0;  // both halves at once: a block has fewer than 2^16 tokens
-      for (int w = group * group_warps; w < (group + 1) * group_warps; ++w) {
-        const uint32_t c = sh.counter[w][word];
-        sh.counter[w][word] = run;
-        run += c;
+      const int word = tid % kWords, half = tid / kWords;
+      uint32_t c[kHalfWarps], run = 0;  // both counters at once: a block has fewer than 2^16 tokens
+#pragma unroll
+      for (int w = 0; w < kHalfWarps; ++w) c[w] = sh.counter[half * kHalfWarps + w][word];
+#pragma unroll
+      for (int w = 0; w < kHalfWarps; ++w) {
+        sh.counter[half * kHalfWarps + w][word] = run;
+        run += c[w];
       }
-      sh.offset[group * words + word] = run;
+      sh.offset[half][word] = run;
     }
     __syncthreads();
-    if (tid < words) {
-      uint32_t run = 0;
-      for (int g = 0; g < groups; ++g) {
-        const uint32_t c = sh.offset[g * words + tid];
-        sh.offset[g * words + tid] = run;
-        run += c;
-      }
-      sh.total[2 * tid] = run & 0xffffu;
-      sh.total[2 * tid + 1] = run >> 16;
-    }
-    cluster.sync();
-    uint32_t all = 0, before = 0;
-    if (tid < radix) {
-      for (int b = 0; b < blocks; ++b) {
-        const uint32_t c = cluster.map_shared_rank(&sh, b)->total[tid];
-        all += c;
-        if (b < block) before += c;
+    // this thread's digit: its total, and where it starts in the block's order
+    uint32_t total = 0;
+    {
+      uint16_t* offset = reinterpret_cast<uint16_t*>(sh.offset);
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) {
+        const uint32_t c = offset[h * kRadix + tid];
+        offset[h * kRadix + tid] = uint16_t(total);
+        total += c;
       }
     }
+    if (blocks > 1) __stcg(a.totals + block * kRadix + tid, total);
     uint32_t sum;
-    const uint32_t first = block_scan(all, sh.warp_sum, &sum);
-    if (tid < radix) sh.base[tid] = first + before;
+    const uint32_t start = block_scan(total, sh.warp_sum, &sum);
+    sh.start[tid] = start;
     __syncthreads();
-    const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset) + (warp / group_warps) * radix;
+    const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset[warp / kHalfWarps]);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & (radix - 1);
-      const uint32_t to = sh.base[d] + offset[d] + count[d] + rank[k];
-      cluster.map_shared_rank(&sh, to / kPart)->item[to % kPart] = mine[k];
+      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1);
+      rank[k] += sh.start[d] + offset[d] + count[d];
+    }
+    __syncthreads();  // the counters are read: their memory takes the tokens
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) sh.local[rank[k]] = mine[k];
+    uint32_t all = total, before = 0;
+    if (blocks > 1) {
+      cluster.sync();
+      uint32_t of[kMaxBlocks];
+#pragma unroll
+      for (int b = 0; b < kMaxBlocks; ++b) of[b] = b < blocks ? __ldcg(a.totals + b * kRadix + tid) : 0;
+      all = 0;
+#pragma unroll
+      for (int b = 0; b < kMaxBlocks; ++b) {
+        all += of[b];
+        before += b < block ? of[b] : 0;
+      }
+    }
+    sh.base[tid] = block_scan(all, sh.warp_sum, &sum) + before - start;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int at = k * kGroupThreads + tid;
+      const uint2 it = sh.local[at];
+      const uint32_t to = sh.base[(it.x >> shift) & (kRadix - 1)] + at;
+      if (to < uint32_t(a.n)) {
+        __stcg(key_to + to, it.x);
+        __stcg(pos_to + to, it.y);
+      }
     }
     cluster.sync();
-    if (p + 1 < a.passes) {
-#pragma unroll
-      for (int k = 0; k < ITEMS; ++k) mine[k] = sh.item[(warp * ITEMS + k) * 32 + lane];
-    }
   }
-  // the tokens in order, and where the rows begin
-  const uint32_t left = block > 0 ? cluster.map_shared_rank(&sh, block - 1)->item[kPart - 1].x : 0xffffffffu;
+  if (!a.place) return;
+  // where the rows begin
   unsigned heads[ITEMS];
+  uint32_t key[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int at = k * kGroupThreads + tid, i = block * kPart + at;
-    const uint2 it = sh.item[at];
-    const uint32_t prev = at > 0 ? sh.item[at - 1].x : left;
-    if (i < a.n) {
-      a.keys[i] = it.x;
-      a.pos[i] = it.y;
-    }
-    heads[k] = __ballot_sync(kFull, it.x < a.vocab && (i == 0 || prev != it.x));
+    const int i = block * kPart + k * kGroupThreads + tid;
+    key[k] = i < a.n ? __ldcg(a.key[0] + i) : 0xffffffffu;
+    const uint32_t prev = i > 0 && i < a.n ? __ldcg(a.key[0] + i - 1) : 0xffffffffu;
+    heads[k] = __ballot_sync(kFull, key[k] < a.vocab && prev != key[k]);
     if (lane == 0) sh.heads[k * kGroupWarps + warp] = __popc(heads[k]);
-  }
-  if (!a.place) {
-    cluster.sync();  // a block's last token is read until here
-    return;
   }
   __syncthreads();
   // heads before each warp's round, in the block
-  const bool mine_counts = tid < kGroupWarps * ITEMS;
+  const bool counts = tid < kGroupWarps * ITEMS;
   uint32_t block_heads;
-  const uint32_t before_me = block_scan(mine_counts ? sh.heads[tid % (kGroupWarps * ITEMS)] : 0, sh.warp_sum, &block_heads);
-  if (mine_counts) sh.heads[tid] = before_me;
-  if (tid == 0) sh.block_heads = block_heads;
+  const uint32_t heads_before = block_scan(counts ? sh.heads[tid % (kGroupWarps * ITEMS)] : 0, sh.warp_sum, &block_heads);
+  if (counts) sh.heads[tid] = heads_before;
+  if (tid == 0) __stcg(a.totals + kMaxBlocks * kRadix + block, block_heads);
   cluster.sync();
   uint32_t before = 0, total = 0;
   for (int b = 0; b < blocks; ++b) {
-    const uint32_t c = cluster.map_shared_rank(&sh, b)->block_heads;
+    const uint32_t c = __ldcg(a.totals + kMaxBlocks * kRadix + b);
     total += c;
     if (b < block) before += c;
   }
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int at = k * kGroupThreads + tid, i = block * kPart + at;
+    const int i = block * kPart + k * kGroupThreads + tid;
     if (i >= a.n) continue;
-    const uint32_t key = sh.item[at].x;
     const uint32_t upto = before + sh.heads[k * kGroupWarps + warp] + __popc(heads[k] & (kFull >> (31 - lane)));
-    if (key < a.vocab) a.place[i] = upto - 1;
-    if (heads[k] >> lane & 1) a.row_ids[upto - 1] = int32_t(key);
+    if (key[k] < a.vocab) a.place[i] = upto - 1;
+    if (heads[k] >> lane & 1) a.row_ids[upto - 1] = int32_t(key[k]);
     if (uint32_t(i) >= total) a.row_ids[i] = -1;
   }
   if (block == 0 && tid == 0) *a.count = int32_t(total);
-  cluster.sync();  // the blocks' counts are read until here
 }
 
 template <int ITEMS>
@@ -752,7 +786,9 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   const int digit = (bits + passes - 1) / passes;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, kChunk);
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
-  const size_t hist = round256(size_t(tiles) * (size_t(1) << digit) * 4);
+  const bool grouped_here = n <= kMaxGroup;
+  const size_t hist = grouped_here ? round256((kMaxBlocks * kRadix + kMaxBlocks) * 4)
+                                   : round256(size_t(tiles) * (size_t(1) << digit) * 4);
   Scratch ws(s);
   FG_TRY(scratch_alloc(&ws.p, 5 * list + hist + 2 * part, s));
   unsigned char* at = static_cast<unsigned char*>(ws.p);
@@ -768,10 +804,9 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   SumArgs a{};
   a.head = static_cast<float*>(take(part));
   a.tail = static_cast<float*>(take(part));
-  const bool grouped_here = n <= kMaxGroup;
   if (n > 0 && grouped_here) {
-    GroupArgs g{ids, int(n), vocab, padding, passes, std::max(digit, kMinDigit), key[0], pos[0], compact ? place : nullptr,
-                row_ids, count, err};
+    GroupArgs g{ids, int(n), vocab, padding, passes, counts, {key[0], key[1]}, {pos[0], pos[1]},
+                compact ? place : nullptr, row_ids, count, err};
     FG_TRY(group_tokens(g, s));
   } else if (n > 0) {
     for (int p = 0; p < passes; ++p) {
