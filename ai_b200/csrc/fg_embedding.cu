@@ -543,6 +543,24 @@ __device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, 
   return lo;
 }
 
+// A kernel launched to overlap the end of the one before it: its blocks may
+// start while that one's last still run, and read nothing until it is done.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t s, const A&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  return FG_OK;
+}
+
 // ------------------------------------------------------------------ sums
 // A warp sums one chunk of sorted tokens over 32·VEC columns, with kAhead
 // rows in flight. A run of one id that lies within the chunk is written as
@@ -564,6 +582,10 @@ struct SumArgs {
   int accumulate;
   float* head;
   float* tail;  // [chunks, dim] each
+  // blocks that zero the rows without tokens, spread among those that sum
+  int64_t rows;
+  const int32_t* count;  // rows met, of the compact gradient; null: the dense one
+  int sum_blocks, zero_blocks;
 };
 
 template <typename TG, int VEC>
@@ -580,10 +602,48 @@ __device__ __forceinline__ void write_row(TG* g, const float (&acc)[VEC], float 
   r.store(g);
 }
 
+// Zeros in the rows of the dense gradient that no token met (there may be
+// no tokens at all), or past the last row of the compact one: a warp takes
+// 32 rows.
+template <typename TG, int VEC>
+__device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t r0, TG* grad, int lane) {
+  if (r0 >= a.rows) return;
+  unsigned met = 0;
+  if (!a.count) {
+    // the sorted tokens of the 32 rows are [lo, hi); each lane looks its row up
+    const int64_t lo = first_token(a.keys, a.n, r0, lane), hi = first_token(a.keys, a.n, r0 + 32, lane);
+    int64_t l = lo, h = hi;
+    while (l < h) {
+      const int64_t mid = (l + h) / 2;
+      if (a.keys[mid] < r0 + lane)
+        l = mid + 1;
+      else
+        h = mid;
+    }
+    met = __ballot_sync(kFull, l < hi && a.keys[l] == r0 + lane);
+  } else {
+    const int64_t c = *a.count;
+    met = c >= r0 + 32 ? kFull : c > r0 ? (1u << (c - r0)) - 1 : 0;
+  }
+  Pack<TG, VEC> z;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
+  for (int r = 0; r < 32 && r0 + r < a.rows; ++r) {
+    if (met >> r & 1) continue;
+    for (int c = lane; c < a.dim / VEC; c += 32) z.store(grad + (r0 + r) * a.ldg + int64_t(c) * VEC);
+  }
+}
+
 template <typename TY, typename TG, int VEC>
 __global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(SumArgs a, const TY* __restrict__ dy, TG* grad) {
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  wait_for_previous();
+  const int64_t zeros = int64_t(blockIdx.x) * a.zero_blocks / (a.sum_blocks + a.zero_blocks);  // before this block
+  if (int64_t(blockIdx.x + 1) * a.zero_blocks / (a.sum_blocks + a.zero_blocks) > zeros) {
+    zero_rows<TG, VEC>(a, (zeros * kSumWarps + warp) * 32, grad, lane);
+    return;
+  }
+  const int64_t unit = (blockIdx.x - zeros) * kSumWarps + warp;
   const int64_t chunk = unit / a.slices;
   const int col = (int(unit % a.slices) * 32 + lane) * VEC;
   const int64_t i0 = chunk * kChunk;
@@ -655,6 +715,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
   const int64_t chunk0 = blockIdx.x % blocks * kSumWarps;
   const int col = (int(blockIdx.x / blocks) * 32 + lane) * VEC;
   const bool in = col < a.dim;
+  wait_for_previous();
   // sum of heads [c, c + count) in order, eight in flight
   auto add_heads = [&](float (&acc)[VEC], int64_t c, int count) {
     if (!in) return;
@@ -719,42 +780,6 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
       finish(acc, chunk);
     }
     __syncthreads();
-  }
-}
-
-// Zeros in the rows of the dense gradient that no token met (count null;
-// there may be no tokens at all), or past the last row of the compact one:
-// a warp takes 32 rows.
-template <typename TG, int VEC>
-__global__ void __launch_bounds__(kSumWarps * 32) zero_rows_kernel(const uint32_t* __restrict__ keys, int64_t n,
-                                                                  const int32_t* __restrict__ count, TG* grad,
-                                                                  int64_t rows, int dim, int64_t ldg) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r0 = (int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5)) * 32;
-  if (r0 >= rows) return;
-  unsigned met = 0;
-  if (!count) {
-    // the sorted tokens of the 32 rows are [lo, hi); each lane looks its row up
-    const int64_t lo = first_token(keys, n, r0, lane), hi = first_token(keys, n, r0 + 32, lane);
-    int64_t l = lo, h = hi;
-    while (l < h) {
-      const int64_t mid = (l + h) / 2;
-      if (keys[mid] < r0 + lane)
-        l = mid + 1;
-      else
-        h = mid;
-    }
-    met = __ballot_sync(kFull, l < hi && keys[l] == r0 + lane);
-  } else {
-    const int64_t c = *count;
-    met = c >= r0 + 32 ? kFull : c > r0 ? (1u << (c - r0)) - 1 : 0;
-  }
-  Pack<TG, VEC> z;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
-  for (int r = 0; r < 32 && r0 + r < rows; ++r) {
-    if (met >> r & 1) continue;
-    for (int c = lane; c < dim / VEC; c += 32) z.store(grad + (r0 + r) * ldg + int64_t(c) * VEC);
   }
 }
 
@@ -837,37 +862,26 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
   const int vec = wide ? 4 : 1;
   a.slices = int(blocks_of(dim, 32 * vec));
-  const int64_t rows = compact ? n : vocab;
+  a.rows = compact ? n : vocab;
+  a.count = count;
+  const int64_t sum_blocks = blocks_of(chunks * a.slices, kSumWarps);
+  const int64_t zero_blocks = accumulate ? 0 : blocks_of(a.rows, 32 * kSumWarps);
+  if (sum_blocks + zero_blocks > INT32_MAX) return set_error(FG_EINVAL, "embedding gradient: too many tokens times columns");
+  if (sum_blocks + zero_blocks == 0) return FG_OK;
+  a.sum_blocks = int(sum_blocks);
+  a.zero_blocks = int(zero_blocks);
+  const unsigned threads = kSumWarps * 32, blocks = unsigned(sum_blocks + zero_blocks);
+  const unsigned join_blocks = unsigned(blocks_of(chunks, kSumWarps) * a.slices);
   return by_dtype(grad_dtype, [&](auto tg) {
     using TG = typename decltype(tg)::type;
     TG* g = static_cast<TG*>(grad);
-    const unsigned zero_blocks = unsigned(blocks_of(rows, 32 * kSumWarps));
-    if (!accumulate && rows > 0) {
-      if (wide)
-        zero_rows_kernel<TG, 4><<<zero_blocks, kSumWarps * 32, 0, s>>>(a.keys, n, count, g, rows, a.dim, ldg);
-      else
-        zero_rows_kernel<TG, 1><<<zero_blocks, kSumWarps * 32, 0, s>>>(a.keys, n, count, g, rows, a.dim, ldg);
-      FG_CUDA_TRY(cudaGetLastError());
-    }
-    if (n == 0) return FG_OK;
-    const unsigned sum_blocks = unsigned(blocks_of(chunks * a.slices, kSumWarps));
     FG_TRY(by_dtype(dy_dtype, [&](auto ty) {
       using TY = typename decltype(ty)::type;
-      const TY* y = static_cast<const TY*>(dy);
-      if (wide)
-        sum_kernel<TY, TG, 4><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, y, g);
-      else
-        sum_kernel<TY, TG, 1><<<sum_blocks, kSumWarps * 32, 0, s>>>(a, y, g);
-      FG_CUDA_TRY(cudaGetLastError());
-      return FG_OK;
+      return launch_after(wide ? sum_kernel<TY, TG, 4> : sum_kernel<TY, TG, 1>, blocks, threads, s, a,
+                          static_cast<const TY*>(dy), g);
     }));
-    const unsigned join_blocks = unsigned(blocks_of(chunks, kSumWarps) * a.slices);
-    if (wide)
-      join_kernel<TG, 4><<<join_blocks, kSumWarps * 32, 0, s>>>(a, g);
-    else
-      join_kernel<TG, 1><<<join_blocks, kSumWarps * 32, 0, s>>>(a, g);
-    FG_CUDA_TRY(cudaGetLastError());
-    return FG_OK;
+    if (n <= kChunk) return FG_OK;  // one chunk: nothing crosses
+    return launch_after(wide ? join_kernel<TG, 4> : join_kernel<TG, 1>, join_blocks, threads, s, a, g);
   });
 }
 
