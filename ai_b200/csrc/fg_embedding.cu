@@ -562,13 +562,15 @@ int launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaSt
 }
 
 // ------------------------------------------------------------------ sums
-// A warp sums one chunk of sorted tokens over 32·VEC columns, with kAhead
-// rows in flight. A run of one id that lies within the chunk is written as
+// A warp sums one chunk of sorted tokens over 32·VEC columns, with kRing
+// rows in flight (4, 6 and 8 of them, with the warps that their registers
+// leave room for, measured alike). A run of one id that lies within the chunk is written as
 // its row; a run that came in from the chunk before leaves its sum in
 // head[chunk], one that goes on into the next chunk (and began here) in
 // tail[chunk].
 constexpr int kChunk = 32;
-constexpr int kAhead = 8;
+constexpr int kRing = 4;
+constexpr int kAhead = 8;  // partial sums in flight where they are joined
 constexpr int kSumWarps = 8;
 
 struct SumArgs {
@@ -635,7 +637,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t r0, TG* grad
 }
 
 template <typename TY, typename TG, int VEC>
-__global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(SumArgs a, const TY* __restrict__ dy, TG* grad) {
+__global__ void __launch_bounds__(kSumWarps * 32, 4) sum_kernel(SumArgs a, const TY* __restrict__ dy, TG* grad) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_previous();
   const int64_t zeros = int64_t(blockIdx.x) * a.zero_blocks / (a.sum_blocks + a.zero_blocks);  // before this block
@@ -648,51 +650,50 @@ __global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(SumArgs a, const TY
   const int col = (int(unit % a.slices) * 32 + lane) * VEC;
   const int64_t i0 = chunk * kChunk;
   if (i0 >= a.n) return;
-  const int count = int(a.n - i0 < kChunk ? a.n - i0 : kChunk);
-  const uint32_t key = lane < count ? a.keys[i0 + lane] : 0xffffffffu;
+  const uint32_t key = i0 + lane < a.n ? a.keys[i0 + lane] : 0xffffffffu;
+  const int count = __popc(__ballot_sync(kFull, key < a.vocab));  // tokens without a row come last
+  if (count == 0) return;
   const uint32_t pos = lane < count ? a.pos[i0 + lane] : 0;
-  const uint32_t to = !a.place ? key : lane < count && key < a.vocab ? a.place[i0 + lane] : 0;
-  const uint32_t before = i0 > 0 ? a.keys[i0 - 1] : 0xffffffffu;
-  const uint32_t after = i0 + count < a.n ? a.keys[i0 + count] : 0xffffffffu;
+  const uint32_t row = lane < count ? (a.place ? a.place[i0 + lane] : key) : 0;
+  const bool came = i0 > 0 && a.keys[i0 - 1] == __shfl_sync(kFull, key, 0);
+  const bool goes = count == kChunk && i0 + kChunk < a.n && a.keys[i0 + kChunk] == __shfl_sync(kFull, key, kChunk - 1);
+  const uint32_t next = __shfl_down_sync(kFull, key, 1);
+  // the last tokens of the runs; those whose sum is only a part of the row's
+  const unsigned ends = __ballot_sync(kFull, lane == count - 1 || (lane < count && next != key));
+  const unsigned heads = came ? ends & -ends : 0, tails = goes ? (1u << (count - 1)) & ~heads : 0;
   const bool in = col < a.dim;
+  const TY* y = dy + col;
+  Pack<TY, VEC> v[kRing];
+  auto load = [&](int u, int t) {
+    const uint32_t from = __shfl_sync(kFull, pos, t & 31);
+    if (t < count && in) v[u].load(y + int64_t(from) * a.ldy);
+  };
+#pragma unroll
+  for (int u = 0; u < kRing; ++u) load(u, u);
   float acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-  bool from_before = true;  // the current run is the chunk's first
-  for (int t0 = 0; t0 < count; t0 += kAhead) {
-    Pack<TY, VEC> v[kAhead];
+  for (int t0 = 0; t0 < count; t0 += kRing) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < kRing; ++u) {
       const int t = t0 + u;
-      const uint32_t k = __shfl_sync(kFull, key, t & 31), p = __shfl_sync(kFull, pos, t & 31);
-      if (t < count && k < a.vocab && in) v[u].load(dy + int64_t(p) * a.ldy + col);
-    }
+      if (t >= count) break;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int t = t0 + u;
-      const uint32_t k = __shfl_sync(kFull, key, t & 31), next = __shfl_sync(kFull, key, (t + 1) & 31);
-      const uint32_t row = __shfl_sync(kFull, to, t & 31);
-      if (t >= count || k >= a.vocab) return;  // tokens without a row come last
-      if (in)
+      for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
+      load(u, t + kRing);
+      if (!(ends >> t & 1)) continue;
+      const uint32_t to = __shfl_sync(kFull, row, t);
+      if (in) {
+        if ((heads | tails) >> t & 1) {
+          float* ws = (heads >> t & 1 ? a.head : a.tail) + chunk * a.dim + col;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
-      const bool last = t == count - 1;
-      if (last || next != k) {
-        const bool came = from_before && before == k;
-        const bool goes = last && after == k;
-        if (in) {
-          if (came || goes) {
-            float* ws = (came ? a.head : a.tail) + chunk * a.dim + col;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) ws[i] = acc[i];
-          } else {
-            write_row<TG, VEC>(grad + int64_t(row) * a.ldg + col, acc, a.scale, a.accumulate);
-          }
+          for (int i = 0; i < VEC; ++i) ws[i] = acc[i];
+        } else {
+          write_row<TG, VEC>(grad + int64_t(to) * a.ldg + col, acc, a.scale, a.accumulate);
         }
-        from_before = false;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
       }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
     }
   }
 }
