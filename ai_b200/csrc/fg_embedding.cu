@@ -491,8 +491,12 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
 template <int ITEMS>
 int launch_group(const GroupArgs& a, int blocks, cudaStream_t s) {
   auto kernel = group_kernel<ITEMS>;
-  FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GroupShared<ITEMS>))));
-  if (blocks > 8) FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  static OncePerDevice ready;
+  if (ready.first()) {
+    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GroupShared<ITEMS>))));
+    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    ready.done();
+  }
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = unsigned(blocks);
@@ -568,7 +572,8 @@ int launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaSt
 // its row; a run that came in from the chunk before leaves its sum in
 // head[chunk], one that goes on into the next chunk (and began here) in
 // tail[chunk].
-constexpr int kChunk = 32;
+constexpr int kMaxChunk = 32;
+constexpr int kMinChunk = 4;
 constexpr int kRing = 4;
 constexpr int kAhead = 8;  // partial sums in flight where they are joined
 constexpr int kSumWarps = 8;
@@ -578,6 +583,7 @@ struct SumArgs {
   const uint32_t* pos;
   const uint32_t* place;  // row of the output for each sorted token; null: its key
   int64_t n, vocab;
+  int chunk;  // tokens of one, a power of two
   int dim, slices;
   int64_t ldy, ldg;
   float scale;
@@ -648,15 +654,16 @@ __global__ void __launch_bounds__(kSumWarps * 32, 4) sum_kernel(SumArgs a, const
   const int64_t unit = (blockIdx.x - zeros) * kSumWarps + warp;
   const int64_t chunk = unit / a.slices;
   const int col = (int(unit % a.slices) * 32 + lane) * VEC;
-  const int64_t i0 = chunk * kChunk;
+  const int size = a.chunk;
+  const int64_t i0 = chunk * size;
   if (i0 >= a.n) return;
-  const uint32_t key = i0 + lane < a.n ? a.keys[i0 + lane] : 0xffffffffu;
+  const uint32_t key = lane < size && i0 + lane < a.n ? a.keys[i0 + lane] : 0xffffffffu;
   const int count = __popc(__ballot_sync(kFull, key < a.vocab));  // tokens without a row come last
   if (count == 0) return;
   const uint32_t pos = lane < count ? a.pos[i0 + lane] : 0;
   const uint32_t row = lane < count ? (a.place ? a.place[i0 + lane] : key) : 0;
   const bool came = i0 > 0 && a.keys[i0 - 1] == __shfl_sync(kFull, key, 0);
-  const bool goes = count == kChunk && i0 + kChunk < a.n && a.keys[i0 + kChunk] == __shfl_sync(kFull, key, kChunk - 1);
+  const bool goes = count == size && i0 + size < a.n && a.keys[i0 + size] == __shfl_sync(kFull, key, size - 1);
   const uint32_t next = __shfl_down_sync(kFull, key, 1);
   // the last tokens of the runs; those whose sum is only a part of the row's
   const unsigned ends = __ballot_sync(kFull, lane == count - 1 || (lane < count && next != key));
@@ -711,7 +718,8 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
   __shared__ int long_run[kSumWarps];
   __shared__ float part[kSumWarps][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chunks = (a.n + kChunk - 1) / kChunk;
+  const int size = a.chunk;
+  const int64_t chunks = (a.n + size - 1) / size;
   const int64_t blocks = (chunks + kSumWarps - 1) / kSumWarps;  // of a slice
   const int64_t chunk0 = blockIdx.x % blocks * kSumWarps;
   const int col = (int(blockIdx.x / blocks) * 32 + lane) * VEC;
@@ -733,12 +741,12 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
     }
   };
   auto finish = [&](const float (&acc)[VEC], int64_t chunk) {
-    const int64_t last = chunk * kChunk + kChunk - 1;
+    const int64_t last = chunk * size + size - 1;
     const int64_t row = a.place ? a.place[last] : a.keys[last];
     if (in) write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
   };
 
-  const int64_t chunk = chunk0 + warp, i0 = chunk * kChunk, end = i0 + kChunk;
+  const int64_t chunk = chunk0 + warp, i0 = chunk * size, end = i0 + size;
   int run = 0;  // chunks after this one that the run which leaves it covers
   if (end < a.n) {
     const uint32_t key = a.keys[end - 1];
@@ -746,7 +754,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
     if (key < a.vocab && a.keys[end] == key && began) {
       // chunks that begin with the key: the last is the run's last
       const int64_t next = first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane);
-      run = int((next + kChunk - 1) / kChunk);
+      run = int((next + size - 1) / size);
     }
   }
   float acc[VEC];
@@ -810,7 +818,14 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   while (bits < 31 && (int64_t(1) << bits) <= vocab) ++bits;  // keys reach vocab itself
   const int passes = (bits + kMaxDigit - 1) / kMaxDigit;
   const int digit = (bits + passes - 1) / passes;
-  const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, kChunk);
+  const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
+  const int slices = int(blocks_of(dim, wide ? 128 : 32));
+  // few tokens are cut into shorter chunks, down to kMinChunk, until there is a
+  // warp for every quarter of an SM's: a chunk's rows arrive kRing at a time
+  // (1024 tokens x 768 bf16: 16 us in chunks of 32, 10 us in chunks of 4)
+  int chunk = kMaxChunk;
+  while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
+  const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
   const bool grouped_here = n <= kMaxGroup;
   const size_t hist = grouped_here ? round256((kMaxBlocks * kRadix + kMaxBlocks) * 4)
@@ -860,9 +875,8 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     rest_ids_kernel<<<unsigned(blocks_of(n, 256)), 256, 0, s>>>(row_ids, n, count);
   }
   FG_CUDA_TRY(cudaGetLastError());
-  const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
-  const int vec = wide ? 4 : 1;
-  a.slices = int(blocks_of(dim, 32 * vec));
+  a.chunk = chunk;
+  a.slices = slices;
   a.rows = compact ? n : vocab;
   a.count = count;
   const int64_t sum_blocks = blocks_of(chunks * a.slices, kSumWarps);
@@ -881,7 +895,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
       return launch_after(wide ? sum_kernel<TY, TG, 4> : sum_kernel<TY, TG, 1>, blocks, threads, s, a,
                           static_cast<const TY*>(dy), g);
     }));
-    if (n <= kChunk) return FG_OK;  // one chunk: nothing crosses
+    if (n <= chunk) return FG_OK;  // one chunk: nothing crosses
     return launch_after(wide ? join_kernel<TG, 4> : join_kernel<TG, 1>, join_blocks, threads, s, a, g);
   });
 }

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kPiece = 8192;      // values of a tensor that a block takes at once
+constexpr int kFewTensors = 64;    // of a small call's launch: arguments are copied at every launch
 constexpr int kMaxTensors = 1000;  // of a launch: 29 bytes each within the 32764 of a kernel's arguments
 
 template <int N>
@@ -138,27 +139,10 @@ __global__ void __launch_bounds__(kNormThreads) clip_kernel(const __grid_constan
   }
 }
 
-}  // namespace
-
-}  // namespace fg
-
-using namespace fg;
-
-extern "C" {
-
-int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,
-                      float max_norm, float* norm, void* stream) {
-  clear_error();
-  if (count < 0 || (count > 0 && (!grads || !sizes || !dtypes))) return set_error(FG_EINVAL, "fg_clip_grad_norm: bad tensor list");
-  if (!(max_norm >= 0.f)) return set_error(FG_EINVAL, "fg_clip_grad_norm: max_norm must be at least 0");
-  if (!norm) return set_error(FG_EINVAL, "fg_clip_grad_norm: null norm");
-  for (int i = 0; i < count; ++i) {
-    if (sizes[i] < 0 || sizes[i] / kPiece > (1 << 28)) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d has %lld values", i, (long long)sizes[i]);
-    if (!known_dtype(dtypes[i])) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d has unknown element type %d", i, dtypes[i]);
-    if (sizes[i] > 0 && (!grads[i] || (outs && !outs[i]))) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d is null", i);
-  }
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int launches = std::max(1, (count + kMaxTensors - 1) / kMaxTensors);
+template <int N>
+int clip_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,
+                   float max_norm, float* norm, cudaStream_t s) {
+  const int launches = std::max(1, (count + N - 1) / N);
   const int blocks = sm_count() * 8;
   void* ws = nullptr;
   FG_TRY(scratch_alloc(&ws, size_t(launches) * blocks * sizeof(double), s));
@@ -166,10 +150,10 @@ int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes,
   int rc = FG_OK;
   for (int pass = 0; pass < 2 && rc == FG_OK; ++pass) {
     for (int l = 0; l < launches && rc == FG_OK; ++l) {
-      TensorList<kMaxTensors> t;
+      TensorList<N> t;
       t.count = 0;
       t.first[0] = 0;
-      for (int i = l * kMaxTensors; i < std::min(count, (l + 1) * kMaxTensors); ++i) {
+      for (int i = l * N; i < std::min(count, (l + 1) * N); ++i) {
         t.in[t.count] = grads[i];
         t.out[t.count] = outs ? outs[i] : const_cast<void*>(grads[i]);
         t.size[t.count] = sizes[i];
@@ -192,6 +176,30 @@ int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes,
   }
   scratch_free(ws, s);
   return rc;
+}
+
+}  // namespace
+
+}  // namespace fg
+
+using namespace fg;
+
+extern "C" {
+
+int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,
+                      float max_norm, float* norm, void* stream) {
+  clear_error();
+  if (count < 0 || (count > 0 && (!grads || !sizes || !dtypes))) return set_error(FG_EINVAL, "fg_clip_grad_norm: bad tensor list");
+  if (!(max_norm >= 0.f)) return set_error(FG_EINVAL, "fg_clip_grad_norm: max_norm must be at least 0");
+  if (!norm) return set_error(FG_EINVAL, "fg_clip_grad_norm: null norm");
+  for (int i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || sizes[i] / kPiece > (1 << 28)) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d has %lld values", i, (long long)sizes[i]);
+    if (!known_dtype(dtypes[i])) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d has unknown element type %d", i, dtypes[i]);
+    if (sizes[i] > 0 && (!grads[i] || (outs && !outs[i]))) return set_error(FG_EINVAL, "fg_clip_grad_norm: tensor %d is null", i);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (count <= kFewTensors) return clip_grad_norm<kFewTensors>(count, grads, sizes, dtypes, outs, max_norm, norm, s);
+  return clip_grad_norm<kMaxTensors>(count, grads, sizes, dtypes, outs, max_norm, norm, s);
 }
 
 }  // extern "C"

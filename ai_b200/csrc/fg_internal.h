@@ -7,6 +7,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -37,6 +38,23 @@ const char* last_error();
 
 // Number of SMs of the current device (cached per device).
 int sm_count();
+
+// A step that each device needs once (a kernel's attributes): first() until
+// done() was called on the current device. Two threads may both take it.
+class OncePerDevice {
+ public:
+  bool first() {
+    int dev = 0;
+    return cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(devices_.load() >> dev & 1);
+  }
+  void done() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev < 64) devices_.fetch_or(uint64_t(1) << dev);
+  }
+
+ private:
+  std::atomic<uint64_t> devices_{0};
+};
 
 // Status block of the current device (error word, then the pipeline-wait
 // limit; fg_ptx.cuh DeviceStatus); kernels record bounded-wait timeouts

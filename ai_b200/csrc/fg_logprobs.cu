@@ -480,7 +480,11 @@ int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
     FG_CUDA_TRY(cudaGetLastError());
     return FG_OK;
   }
-  if (split > 8) FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  static OncePerDevice ready;
+  if (split > 8 && ready.first()) {
+    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    ready.done();
+  }
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = unsigned(split);

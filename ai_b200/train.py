@@ -28,14 +28,15 @@ from .tensor import TensorError, _fail
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
-def _run(name: str, device: torch.device, *args) -> None:
-    """Calls an entry point on the device's current stream, its last argument."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+def _run(name: str, index: int, *args) -> None:
+    """Calls an entry point of the library on device `index`, with that
+    device's current stream as the last argument."""
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream without its object
+    if torch.cuda.current_device() == index:
         rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, stream)
     if rc:
         _lib.check(rc)
@@ -48,27 +49,30 @@ def _dtype(op: str, name: str, t: torch.Tensor) -> int:
     return code
 
 
-def _int32(op: str, name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
-        _fail(op, f"{name} must be an int32 tensor on {device}")
-    return t.contiguous()
+def _int32(op: str, name: str, t: torch.Tensor, index: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.get_device() != index:
+        _fail(op, f"{name} must be an int32 tensor on cuda:{index}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _float32(op: str, name: str, t: torch.Tensor, rows: int, device: torch.device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or t.numel() != rows:
-        _fail(op, f"{name} must be {rows} float32 values on {device}")
-    return t.contiguous()
+def _float32(op: str, name: str, t: torch.Tensor, rows: int, index: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != index or t.numel() != rows:
+        _fail(op, f"{name} must be {rows} float32 values on cuda:{index}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous rows at a stride of at least their length."""
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1] and t.shape[0] > 1:
-        return t.contiguous()
-    return t
+def _stride(t: torch.Tensor, rows: int, cols: int) -> int:
+    """The distance of t's rows, 0 where they are not contiguous or overlap."""
+    s0, s1 = t.stride()
+    if s1 != 1 and cols > 1 or s0 < cols and rows > 1:
+        return 0
+    return s0 if s0 > cols else cols
 
 
-def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+def _rows(t: torch.Tensor, rows: int, cols: int):
+    """t with contiguous rows, and their distance."""
+    ld = _stride(t, rows, cols)
+    return (t, ld) if ld else (t.contiguous(), cols)
 
 
 def Check(device=None) -> None:
@@ -85,34 +89,42 @@ def Embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     ``padding`` has a zero row; -1 stands for empty slots."""
     op = "Embedding"
     code = _dtype(op, "table", table)
-    if table.dim() != 2 or table.shape[1] == 0:
-        _fail(op, f"table must be 2-D, got {list(table.shape)}")
-    dtype = table.dtype if dtype is None else dtype
-    if dtype not in _DTYPES:
+    shape = table.shape
+    if len(shape) != 2 or shape[1] == 0:
+        _fail(op, f"table must be 2-D, got {list(shape)}")
+    vocab, dim = shape
+    if dtype is None:
+        dtype = table.dtype
+    out_code = _DTYPES.get(dtype)
+    if out_code is None:
         _fail(op, f"no output type {dtype}")
-    ids = _int32(op, "ids", ids, table.device)
-    table = _rows(table)
-    vocab, dim = table.shape
-    out = torch.empty((*ids.shape, dim), dtype=dtype, device=table.device)
-    _run("fg_embedding", table.device, table.data_ptr(), code, vocab, dim, _ld(table), ids.data_ptr(), ids.numel(),
-         scale, padding, out.data_ptr(), _DTYPES[dtype], dim)
+    index = table.get_device()
+    ids = _int32(op, "ids", ids, index)
+    table, ld = _rows(table, vocab, dim)
+    out = table.new_empty((*ids.shape, dim), dtype=dtype)
+    _run("fg_embedding", index, table.data_ptr(), code, vocab, dim, ld, ids.data_ptr(), ids.numel(), scale, padding,
+         out.data_ptr(), out_code, dim)
     return out
 
 
 def _grad_args(op: str, dy: torch.Tensor, ids: torch.Tensor, vocab: int, dtype: Optional[torch.dtype]):
     code = _dtype(op, "dy", dy)
-    if dy.dim() < 2 or dy.shape[-1] == 0:
-        _fail(op, f"dy must be [tokens, dim], got {list(dy.shape)}")
-    ids = _int32(op, "ids", ids, dy.device)
-    if dy.shape[:-1] != ids.shape:
-        _fail(op, f"dy {list(dy.shape)} does not match ids {list(ids.shape)}")
+    shape = dy.shape
+    if len(shape) < 2 or shape[-1] == 0:
+        _fail(op, f"dy must be [tokens, dim], got {list(shape)}")
+    index = dy.get_device()
+    ids = _int32(op, "ids", ids, index)
+    if shape[:-1] != ids.shape:
+        _fail(op, f"dy {list(shape)} does not match ids {list(ids.shape)}")
     if vocab < 0:
         _fail(op, f"vocabulary of {vocab}")
     if dtype is not None and dtype not in _DTYPES:
         _fail(op, f"no output type {dtype}")
-    if dy.dim() != 2:
-        dy = dy.reshape(-1, dy.shape[-1])
-    return code, _rows(dy), ids
+    if len(shape) != 2:
+        dy = dy.reshape(-1, shape[-1])
+    n, dim = ids.numel(), shape[-1]
+    dy, ld = _rows(dy, n, dim)
+    return code, dy, ld, ids, n, dim, index
 
 
 def EmbeddingGrad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float = 1.0, padding: int = -1,
@@ -123,23 +135,20 @@ def EmbeddingGrad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
     added to it with ``accumulate`` (then rows without a token are not
     touched); otherwise a new tensor of ``dtype`` (dy's where None)."""
     op = "EmbeddingGrad"
-    code, dy, ids = _grad_args(op, dy, ids, vocab, dtype)
-    dim = dy.shape[1]
+    code, dy, ld, ids, n, dim, index = _grad_args(op, dy, ids, vocab, dtype)
     if out is None:
         if accumulate:
             _fail(op, "accumulate needs out")
-        out_dtype = dy.dtype if dtype is None else dtype
+        out, ldo = dy.new_empty((vocab, dim), dtype=dtype), dim
     else:
         _dtype(op, "out", out)
-        if out.device != dy.device or tuple(out.shape) != (vocab, dim) or dtype not in (None, out.dtype):
-            _fail(op, f"out must be [{vocab}, {dim}] on {dy.device}, got {out.dtype} {list(out.shape)}")
-        if out.stride(1) != 1 and dim > 1 or out.stride(0) < dim and vocab > 1:
+        if out.get_device() != index or tuple(out.shape) != (vocab, dim) or dtype not in (None, out.dtype):
+            _fail(op, f"out must be [{vocab}, {dim}] on cuda:{index}, got {out.dtype} {list(out.shape)}")
+        ldo = _stride(out, vocab, dim)
+        if not ldo:
             _fail(op, "out must have contiguous rows")
-        out_dtype = out.dtype
-    if out is None:
-        out = torch.empty((vocab, dim), dtype=out_dtype, device=dy.device)
-    _run("fg_embedding_grad", dy.device, dy.data_ptr(), code, _ld(dy), ids.data_ptr(), ids.numel(), vocab, dim, scale,
-         padding, out.data_ptr(), _DTYPES[out_dtype], _ld(out), int(accumulate))
+    _run("fg_embedding_grad", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding,
+         out.data_ptr(), _DTYPES[out.dtype], ldo, int(accumulate))
     return out
 
 
@@ -156,14 +165,12 @@ def EmbeddingGradRows(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: fl
     """``EmbeddingGrad``'s rows that have tokens, on the device without a
     synchronisation: room for as many rows as there are tokens."""
     op = "EmbeddingGradRows"
-    code, dy, ids = _grad_args(op, dy, ids, vocab, dtype)
-    n, dim = dy.shape
-    out_dtype = dy.dtype if dtype is None else dtype
-    row_ids = torch.empty(n + 1, dtype=torch.int32, device=dy.device)
-    rows = torch.empty((n, dim), dtype=out_dtype, device=dy.device)
+    code, dy, ld, ids, n, dim, index = _grad_args(op, dy, ids, vocab, dtype)
+    row_ids = ids.new_empty(n + 1)
+    rows = dy.new_empty((n, dim), dtype=dtype)
     at = row_ids.data_ptr()
-    _run("fg_embedding_grad_rows", dy.device, dy.data_ptr(), code, _ld(dy), ids.data_ptr(), n, vocab, dim, scale,
-         padding, at, rows.data_ptr(), _DTYPES[out_dtype], dim, at + 4 * n)
+    _run("fg_embedding_grad_rows", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding, at,
+         rows.data_ptr(), _DTYPES[rows.dtype], dim, at + 4 * n)
     return RowsGrad(row_ids[:n], rows, row_ids[n:])
 
 
@@ -179,14 +186,18 @@ class LogProbsResult(NamedTuple):
 
 def _logits(op: str, logits: torch.Tensor, targets: torch.Tensor, scale: float):
     code = _dtype(op, "logits", logits)
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        _fail(op, f"logits must be [rows, width], got {list(logits.shape)}")
-    targets = _int32(op, "targets", targets, logits.device)
-    if targets.numel() != logits.shape[0]:
-        _fail(op, f"{targets.numel()} targets for {logits.shape[0]} rows")
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0:
+        _fail(op, f"logits must be [rows, width], got {list(shape)}")
+    rows, width = shape
+    index = logits.get_device()
+    targets = _int32(op, "targets", targets, index)
+    if targets.numel() != rows:
+        _fail(op, f"{targets.numel()} targets for {rows} rows")
     if not 0 < scale < float("inf"):
         _fail(op, f"scale {scale} must be positive and finite")
-    return code, _rows(logits), targets
+    logits, ld = _rows(logits, rows, width)
+    return code, logits, ld, targets, rows, width, index
 
 
 def LogProbs(logits: torch.Tensor, targets: torch.Tensor, scale: float = 1.0, top: int = 0) -> LogProbsResult:
@@ -194,20 +205,18 @@ def LogProbs(logits: torch.Tensor, targets: torch.Tensor, scale: float = 1.0, to
     target is negative), with the rows' entropies, log sums and ``top`` most
     probable columns (equal logits by ascending index)."""
     op = "LogProbs"
-    code, logits, targets = _logits(op, logits, targets, scale)
-    rows, width = logits.shape
+    code, logits, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
     if not 0 <= top <= min(width, _lib.MAX_TOP):
         _fail(op, f"{top} alternatives of {width} columns (at most {_lib.MAX_TOP})")
-    out = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
+    out = logits.new_empty((3, rows), dtype=torch.float32)
     at = out.data_ptr()
-    index = value = None
+    place = value = place_at = value_at = None
     if top:
-        index = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        value = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    _run("fg_log_probs", logits.device, logits.data_ptr(), code, rows, width, _ld(logits), targets.data_ptr(), scale,
-         top, at, at + 4 * rows, at + 8 * rows, index.data_ptr() if top else None, value.data_ptr() if top else None)
-    logprob, entropy, lse = out
-    return LogProbsResult(logprob, entropy, lse, index, value)
+        place, value = targets.new_empty((rows, top)), out.new_empty((rows, top))
+        place_at, value_at = place.data_ptr(), value.data_ptr()
+    _run("fg_log_probs", index, logits.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, top, at,
+         at + 4 * rows, at + 8 * rows, place_at, value_at)
+    return LogProbsResult(*out.unbind(), place, value)
 
 
 def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, dlogprob: torch.Tensor,
@@ -217,25 +226,26 @@ def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
     the gradients of its log probabilities and, where ``dentropy`` is given,
     of its entropies. ``out`` may be the logits themselves."""
     op = "LogProbsGrad"
-    code, x, targets = _logits(op, logits, targets, scale)
-    rows, width = x.shape
-    lse = _float32(op, "lse", lse, rows, x.device)
-    dlogprob = _float32(op, "dlogprob", dlogprob, rows, x.device)
+    code, x, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
+    lse = _float32(op, "lse", lse, rows, index)
+    dlogprob = _float32(op, "dlogprob", dlogprob, rows, index)
+    entropy_at = dentropy_at = None
     if dentropy is not None:
-        dentropy = _float32(op, "dentropy", dentropy, rows, x.device)
+        dentropy = _float32(op, "dentropy", dentropy, rows, index)
         if entropy is None:
             _fail(op, "dentropy needs entropy")
-        entropy = _float32(op, "entropy", entropy, rows, x.device)
-    if out is not None:
-        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != x.device or out.shape != x.shape:
-            _fail(op, f"out must be {x.dtype} [{rows}, {width}] on {x.device}")
-        if out.stride(1) != 1 and width > 1 or out.stride(0) < width and rows > 1:
-            _fail(op, "out must have contiguous rows")
+        entropy = _float32(op, "entropy", entropy, rows, index)
+        entropy_at, dentropy_at = entropy.data_ptr(), dentropy.data_ptr()
     if out is None:
-        out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    _run("fg_log_probs_grad", x.device, x.data_ptr(), code, rows, width, _ld(x), targets.data_ptr(), scale,
-         lse.data_ptr(), None if dentropy is None else entropy.data_ptr(), dlogprob.data_ptr(),
-         None if dentropy is None else dentropy.data_ptr(), out.data_ptr(), _ld(out))
+        out, ldo = x.new_empty((rows, width)), width
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.get_device() != index or out.shape != x.shape:
+            _fail(op, f"out must be {x.dtype} [{rows}, {width}] on cuda:{index}")
+        ldo = _stride(out, rows, width)
+        if not ldo:
+            _fail(op, "out must have contiguous rows")
+    _run("fg_log_probs_grad", index, x.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, lse.data_ptr(),
+         entropy_at, dlogprob.data_ptr(), dentropy_at, out.data_ptr(), ldo)
     return out
 
 
@@ -252,20 +262,21 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
     n = len(grads)
     if n == 0:
         _fail(op, "no gradients")
-    device = grads[0].device
     try:
         codes = [_DTYPES[g.dtype] for g in grads]
+        index = grads[0].get_device()
+        alike = index >= 0 and all([g.get_device() == index and g.is_contiguous() for g in grads])
     except (KeyError, AttributeError):
         _fail(op, "gradients must be float32, bfloat16 or float16 tensors")
-    if not all([g.device == device and g.is_contiguous() for g in grads]) or device.type != "cuda":
+    if not alike:
         _fail(op, "gradients must be contiguous tensors on one CUDA device")
     outs = None
     if out is not None:
-        if len(out) != n or not all([o.dtype == g.dtype and o.shape == g.shape and o.device == device and
+        if len(out) != n or not all([o.dtype == g.dtype and o.shape == g.shape and o.get_device() == index and
                                      o.is_contiguous() for o, g in zip(out, grads)]):
             _fail(op, "out must match the gradients' shapes, types and device, contiguous")
         outs = (C.c_void_p * n)(*[o.data_ptr() for o in out])
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    _run("fg_clip_grad_norm", device, n, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    _run("fg_clip_grad_norm", index, n, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
          (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int * n)(*codes), outs, max_norm, norm.data_ptr())
     return norm
