@@ -257,6 +257,15 @@ __global__ void __launch_bounds__(kSortThreads) heads_place_kernel(const uint32_
   }
 }
 
+// Sets the bit of every row that a token met.
+__global__ void __launch_bounds__(kSortThreads) met_kernel(const uint32_t* __restrict__ keys, int64_t n, int64_t vocab,
+                                                          uint32_t* __restrict__ met) {
+  const int64_t i = int64_t(blockIdx.x) * kSortThreads + threadIdx.x;
+  if (i >= n) return;
+  const uint32_t key = keys[i];
+  if (key < vocab && (i == 0 || keys[i - 1] != key)) atomicOr(met + key / 32, 1u << key % 32);
+}
+
 __global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* count) {
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i < n && i >= *count) row_ids[i] = -1;
@@ -288,10 +297,11 @@ struct GroupArgs {
   const int32_t* ids;
   int n;
   int64_t vocab;
-  int padding, passes;
+  int padding, passes, digit;
   uint32_t* totals;  // [kMaxBlocks, kRadix] and kMaxBlocks more
   uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
   uint32_t* pos[2];
+  uint32_t* met;     // a bit for every row, set where a token met it; null: not asked for
   uint32_t* place;   // with row_ids and count: the rows met; null: not asked for
   int32_t* row_ids;
   int32_t* count;
@@ -341,6 +351,9 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = gridDim.x, block = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t mask = (1u << a.digit) - 1;
+  if (a.met)  // the barriers of the passes come before the first bit is set
+    for (int64_t i = block * kGroupThreads + tid; i < (a.vocab + 31) / 32; i += blocks * kGroupThreads) __stcg(a.met + i, 0u);
   uint2 mine[ITEMS];  // (key, position) of consecutive tokens of a warp, 32 a round
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
@@ -351,10 +364,14 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   for (int k = 0; k < ITEMS; ++k)  // places past the last token sort behind every key
     mine[k].x = int(mine[k].y) < a.n ? token_key(int(mine[k].x), a.vocab, a.padding, a.err) : 0xffffffffu;
   for (int p = 0; p < a.passes; ++p) {
-    const int shift = p * kMaxDigit;
+    const int shift = p * a.digit;
     uint32_t* key_to = a.key[(a.passes - 1 - p) & 1];
     uint32_t* pos_to = a.pos[(a.passes - 1 - p) & 1];
-    if (p > 0) {
+    if (p > 0 && blocks == 1) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) mine[k] = sh.local[(warp * ITEMS + k) * 32 + lane];
+      __syncthreads();
+    } else if (p > 0) {
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k) {
         const int i = block * kPart + (warp * ITEMS + k) * 32 + lane;
@@ -370,10 +387,11 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     uint32_t rank[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1);
+      const uint32_t d = (mine[k].x >> shift) & mask;
       unsigned same = kFull;
 #pragma unroll
       for (int b = 0; b < kMaxDigit; ++b) {
+        if (b == a.digit) break;
         const bool set = d >> b & 1;
         const unsigned vote = __ballot_sync(kFull, set);
         same &= set ? vote : ~vote;
@@ -417,12 +435,16 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset[warp / kHalfWarps]);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1);
+      const uint32_t d = (mine[k].x >> shift) & mask;
       rank[k] += sh.start[d] + offset[d] + count[d];
     }
     __syncthreads();  // the counters are read: their memory takes the tokens
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) sh.local[rank[k]] = mine[k];
+    if (blocks == 1 && p + 1 < a.passes) {  // the block's order is the pass's
+      __syncthreads();
+      continue;
+    }
     uint32_t all = total, before = 0;
     if (blocks > 1) {
       cluster.sync();
@@ -442,7 +464,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     for (int k = 0; k < ITEMS; ++k) {
       const int at = k * kGroupThreads + tid;
       const uint2 it = sh.local[at];
-      const uint32_t to = sh.base[(it.x >> shift) & (kRadix - 1)] + at;
+      const uint32_t to = sh.base[(it.x >> shift) & mask] + at;
       if (to < uint32_t(a.n)) {
         __stcg(key_to + to, it.x);
         __stcg(pos_to + to, it.y);
@@ -450,7 +472,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     }
     cluster.sync();
   }
-  if (!a.place) return;
   // where the rows begin
   unsigned heads[ITEMS];
   uint32_t key[ITEMS];
@@ -461,7 +482,9 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     const uint32_t prev = i > 0 && i < a.n ? __ldcg(a.key[0] + i - 1) : 0xffffffffu;
     heads[k] = __ballot_sync(kFull, key[k] < a.vocab && prev != key[k]);
     if (lane == 0) sh.heads[k * kGroupWarps + warp] = __popc(heads[k]);
+    if (a.met && heads[k] >> lane & 1) atomicOr(a.met + key[k] / 32, 1u << key[k] % 32);
   }
+  if (!a.place) return;
   __syncthreads();
   // heads before each warp's round, in the block
   const bool counts = tid < kGroupWarps * ITEMS;
@@ -516,9 +539,10 @@ int launch_group(const GroupArgs& a, int blocks, cudaStream_t s) {
 constexpr int64_t kMaxGroup = int64_t(kMaxBlocks) * kGroupThreads * kMaxGroupItems;
 
 int group_tokens(const GroupArgs& a, cudaStream_t s) {
+  // one block while four tokens a thread will do (nothing is exchanged), then
   // as many blocks as the tokens fill, then more tokens a thread
   int blocks = 1, items = 1;
-  while (blocks < kMaxBlocks && blocks * kGroupThreads < a.n) blocks *= 2;
+  while (a.n > 4 * kGroupThreads && blocks < kMaxBlocks && blocks * kGroupThreads < a.n) blocks *= 2;
   while (int64_t(blocks) * kGroupThreads * items < a.n) items *= 2;
   switch (items) {
     case 1: return launch_group<1>(a, blocks, s);
@@ -593,6 +617,7 @@ struct SumArgs {
   // blocks that zero the rows without tokens, spread among those that sum
   int64_t rows;
   const int32_t* count;  // rows met, of the compact gradient; null: the dense one
+  const uint32_t* met;   // a bit for every row of the dense one; null: no tokens
   int sum_blocks, zero_blocks;
 };
 
@@ -612,34 +637,22 @@ __device__ __forceinline__ void write_row(TG* g, const float (&acc)[VEC], float 
 
 // Zeros in the rows of the dense gradient that no token met (there may be
 // no tokens at all), or past the last row of the compact one: a warp takes
-// 32 rows.
+// 32·VEC columns of 32 rows.
 template <typename TG, int VEC>
-__device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t r0, TG* grad, int lane) {
-  if (r0 >= a.rows) return;
-  unsigned met = 0;
-  if (!a.count) {
-    // the sorted tokens of the 32 rows are [lo, hi); each lane looks its row up
-    const int64_t lo = first_token(a.keys, a.n, r0, lane), hi = first_token(a.keys, a.n, r0 + 32, lane);
-    int64_t l = lo, h = hi;
-    while (l < h) {
-      const int64_t mid = (l + h) / 2;
-      if (a.keys[mid] < r0 + lane)
-        l = mid + 1;
-      else
-        h = mid;
-    }
-    met = __ballot_sync(kFull, l < hi && a.keys[l] == r0 + lane);
-  } else {
-    const int64_t c = *a.count;
-    met = c >= r0 + 32 ? kFull : c > r0 ? (1u << (c - r0)) - 1 : 0;
-  }
+__device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t unit, TG* grad, int lane) {
+  const int64_t r0 = unit / a.slices * 32;
+  const int col = (int(unit % a.slices) * 32 + lane) * VEC;
+  if (r0 >= a.rows || col >= a.dim) return;
+  const int64_t count = a.count ? int64_t(*a.count) - r0 : 0;
+  unsigned keep = a.count ? (count >= 32 ? kFull : count > 0 ? (1u << count) - 1 : 0) : a.met ? a.met[r0 / 32] : 0;
+  if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
   Pack<TG, VEC> z;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
-  for (int r = 0; r < 32 && r0 + r < a.rows; ++r) {
-    if (met >> r & 1) continue;
-    for (int c = lane; c < a.dim / VEC; c += 32) z.store(grad + (r0 + r) * a.ldg + int64_t(c) * VEC);
-  }
+  TG* g = grad + r0 * a.ldg + col;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r)
+    if (!(keep >> r & 1)) z.store(g + r * a.ldg);
 }
 
 template <typename TY, typename TG, int VEC>
@@ -648,7 +661,7 @@ __global__ void __launch_bounds__(kSumWarps * 32, 4) sum_kernel(SumArgs a, const
   wait_for_previous();
   const int64_t zeros = int64_t(blockIdx.x) * a.zero_blocks / (a.sum_blocks + a.zero_blocks);  // before this block
   if (int64_t(blockIdx.x + 1) * a.zero_blocks / (a.sum_blocks + a.zero_blocks) > zeros) {
-    zero_rows<TG, VEC>(a, (zeros * kSumWarps + warp) * 32, grad, lane);
+    zero_rows<TG, VEC>(a, zeros * kSumWarps + warp, grad, lane);
     return;
   }
   const int64_t unit = (blockIdx.x - zeros) * kSumWarps + warp;
@@ -826,12 +839,14 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   int chunk = kMaxChunk;
   while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
+  const bool bits_of_rows = !compact && !accumulate && n > 0;
+  const size_t met_bytes = bits_of_rows ? round256(size_t(blocks_of(vocab, 32)) * 4) : 0;
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
   const bool grouped_here = n <= kMaxGroup;
   const size_t hist = grouped_here ? round256((kMaxBlocks * kRadix + kMaxBlocks) * 4)
                                    : round256(size_t(tiles) * (size_t(1) << digit) * 4);
   Scratch ws(s);
-  FG_TRY(scratch_alloc(&ws.p, 5 * list + hist + 2 * part, s));
+  FG_TRY(scratch_alloc(&ws.p, 5 * list + hist + 2 * part + met_bytes, s));
   unsigned char* at = static_cast<unsigned char*>(ws.p);
   auto take = [&](size_t bytes) {
     void* r = at;
@@ -842,11 +857,13 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   uint32_t* pos[2] = {static_cast<uint32_t*>(take(list)), static_cast<uint32_t*>(take(list))};
   uint32_t* place = static_cast<uint32_t*>(take(list));
   uint32_t* counts = static_cast<uint32_t*>(take(hist));
+  uint32_t* met = bits_of_rows ? static_cast<uint32_t*>(take(met_bytes)) : nullptr;
   SumArgs a{};
+  a.met = met;
   a.head = static_cast<float*>(take(part));
   a.tail = static_cast<float*>(take(part));
   if (n > 0 && grouped_here) {
-    GroupArgs g{ids, int(n), vocab, padding, passes, counts, {key[0], key[1]}, {pos[0], pos[1]},
+    GroupArgs g{ids, int(n), vocab, padding, passes, digit, counts, {key[0], key[1]}, {pos[0], pos[1]}, met,
                 compact ? place : nullptr, row_ids, count, err};
     FG_TRY(group_tokens(g, s));
   } else if (n > 0) {
@@ -867,6 +884,10 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.ldg = ldg;
   a.scale = scale;
   a.accumulate = accumulate;
+  if (met && !grouped_here) {
+    FG_CUDA_TRY(cudaMemsetAsync(met, 0, met_bytes, s));
+    met_kernel<<<unsigned(blocks_of(n, kSortThreads)), kSortThreads, 0, s>>>(a.keys, n, vocab, met);
+  }
   if (compact) a.place = place;
   if (compact && !grouped_here) {
     heads_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts);
@@ -880,7 +901,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.rows = compact ? n : vocab;
   a.count = count;
   const int64_t sum_blocks = blocks_of(chunks * a.slices, kSumWarps);
-  const int64_t zero_blocks = accumulate ? 0 : blocks_of(a.rows, 32 * kSumWarps);
+  const int64_t zero_blocks = accumulate ? 0 : blocks_of(blocks_of(a.rows, 32) * slices, kSumWarps);
   if (sum_blocks + zero_blocks > INT32_MAX) return set_error(FG_EINVAL, "embedding gradient: too many tokens times columns");
   if (sum_blocks + zero_blocks == 0) return FG_OK;
   a.sum_blocks = int(sum_blocks);
