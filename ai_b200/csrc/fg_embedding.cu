@@ -762,12 +762,12 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
   const int64_t chunk = chunk0 + warp, i0 = chunk * size, end = i0 + size;
   int run = 0;  // chunks after this one that the run which leaves it covers
   if (end < a.n) {
-    const uint32_t key = a.keys[end - 1];
-    const bool began = a.keys[i0] != key || i0 == 0 || a.keys[i0 - 1] != key;
-    if (key < a.vocab && a.keys[end] == key && began) {
-      // chunks that begin with the key: the last is the run's last
-      const int64_t next = first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane);
-      run = int((next + size - 1) / size);
+    // the places asked for in one go: the chunk's ends, the next 32 chunks' starts
+    const int64_t start = end + int64_t(lane) * size;
+    const uint32_t key = a.keys[end - 1], first = a.keys[i0], left = i0 > 0 ? a.keys[i0 - 1] : 0xffffffffu;
+    const unsigned same = __ballot_sync(kFull, start < a.n && a.keys[start] == key);
+    if (key < a.vocab && (same & 1) && !(first == key && left == key)) {
+      run = same == kFull ? int((first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane) + size - 1) / size) : __ffs(~same) - 1;
     }
   }
   float acc[VEC];
