@@ -143,8 +143,7 @@ SIGNATURES = {
                                _vp, _vp]),
     "fg_log_probs_grad": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp,
                                     _i64, _vp]),
-    "fg_clip_grad_norm": (C.c_int, [C.c_int, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(C.c_int),
-                                    C.POINTER(_vp), C.c_float, _vp, _vp]),
+    "fg_clip_grad_norm": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp]),
 }
 
 

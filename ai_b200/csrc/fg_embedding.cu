@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "fg_kernels.cuh"
+#include "fg_launch.cuh"
 #include "fg_ptx.cuh"
 #include "fg_types.cuh"
 
@@ -569,24 +570,6 @@ __device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, 
     }
   }
   return lo;
-}
-
-// A kernel launched to overlap the end of the one before it: its blocks may
-// start while that one's last still run, and read nothing until it is done.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-template <typename... P, typename... A>
-int launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t s, const A&... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
-  return FG_OK;
 }
 
 // ------------------------------------------------------------------ sums

@@ -17,7 +17,7 @@ is skipped, and reported by ``Check``. Shape and type errors raise
 """
 from __future__ import annotations
 
-import ctypes as C
+from array import array
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -270,13 +270,16 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
         _fail(op, "gradients must be float32, bfloat16 or float16 tensors")
     if not alike:
         _fail(op, "gradients must be contiguous tensors on one CUDA device")
-    outs = None
+    sizes = [g.numel() for g in grads]
+    outs = outs_at = None
     if out is not None:
-        if len(out) != n or not all([o.dtype == g.dtype and o.shape == g.shape and o.get_device() == index and
-                                     o.is_contiguous() for o, g in zip(out, grads)]):
-            _fail(op, "out must match the gradients' shapes, types and device, contiguous")
-        outs = (C.c_void_p * n)(*[o.data_ptr() for o in out])
+        if len(out) != n or not all([o.dtype == g.dtype and o.numel() == size and o.get_device() == index and
+                                     o.is_contiguous() for o, g, size in zip(out, grads, sizes)]):
+            _fail(op, "out must match the gradients' sizes, types and device, contiguous")
+        outs = array("Q", [o.data_ptr() for o in out])
+        outs_at = outs.buffer_info()[0]
+    ins, sizes, codes = array("Q", [g.data_ptr() for g in grads]), array("q", sizes), array("i", codes)
     norm = grads[0].new_empty((), dtype=torch.float32)
-    _run("fg_clip_grad_norm", index, n, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
-         (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int * n)(*codes), outs, max_norm, norm.data_ptr())
+    _run("fg_clip_grad_norm", index, n, ins.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], outs_at,
+         max_norm, norm.data_ptr())
     return norm
