@@ -159,14 +159,14 @@ __device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
 // bound comes from the first tile: the top-th largest of the lanes' maxima
 // (of half a lane's entries each past 32); a tile with many entries above the
 // bound gives another one in the same way before any is taken. The warps of
-// a block tell one another their bounds. At the end the lists are joined by
-// counting, for every entry, the entries above it.
+// a block tell one another their bounds. At the end the lists are joined two
+// by two, in the block and then by the cluster's first block.
 constexpr int kItems = 16;
 constexpr int kMany = 24;      // lanes with entries above the bound that ask for another bound first
 constexpr int kFew = 3;        // entries that are put in their places one by one
 constexpr int kMaxSplit = 16;  // blocks of a cluster
-constexpr int kMaxWarps = 8;   // of a block
-static_assert(kMaxWarps <= kMaxSplit, "the list has room for either");
+constexpr int kMaxWarps = 16;  // of a block
+static_assert(kMaxSplit <= kMaxWarps, "a warp for every part of a row");
 
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
@@ -195,14 +195,39 @@ struct TopKeys {
     for (int bit = 16; bit > 0; bit >>= 1) x = exchange(x, bit, true, lane);
     return x;
   }
-  // Takes in one key a lane.
-  __device__ __forceinline__ void merge(uint64_t x, int lane) {
-    // rising over the lanes, so that the larger of each lane's two are the
-    // first 32 of both, in an order that `fall` makes descending
+  // Takes in another warp's list.
+  __device__ __forceinline__ void join(const TopKeys& o, int lane) {
+    if (N == 1) {
+      key[0] = fall(larger(key[0], __shfl_sync(kFull, o.key[0], 31 - lane)), lane);
+    } else {
+      const uint64_t a = larger(key[0], __shfl_sync(kFull, o.key[N - 1], 31 - lane));
+      const uint64_t b = larger(key[N - 1], __shfl_sync(kFull, o.key[0], 31 - lane));
+      key[0] = fall(larger(a, b), lane);
+      key[N - 1] = fall(a < b ? a : b, lane);
+    }
+  }
+  __device__ __forceinline__ void load(const uint64_t* p, int lane) {
 #pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
+    for (int n = 0; n < N; ++n) key[n] = p[32 * n + lane];
+  }
+  __device__ __forceinline__ void store(uint64_t* p, int lane) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[32 * n + lane] = key[n];
+  }
+  // Takes in the keys of the first n lanes; the others' are 0.
+  __device__ __forceinline__ void merge(uint64_t x, int n, int lane) {
+    // rising over the lanes, so that the larger of each lane's two are the
+    // first 32 of both, in an order that `fall` makes descending; few keys are
+    // sorted among few lanes and moved behind the zeros
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1) {
 #pragma unroll
       for (int bit = size / 2; bit > 0; bit >>= 1) x = exchange(x, bit, (lane & size) != 0, lane);
+      if (size >= 8 && size < 32 && n <= size) {
+        x = __shfl_sync(kFull, x, (lane + size) & 31);
+        break;
+      }
+    }
     key[N - 1] = fall(larger(key[N - 1], x), lane);
     if (N == 2) {
       const uint64_t rising = __shfl_sync(kFull, key[N - 1], 31 - lane);
@@ -223,26 +248,26 @@ struct TopKeys {
 
 template <int WARPS>
 struct RowShared {
-  uint64_t list[WARPS == kMaxWarps ? kMaxSplit * kMaxTop : WARPS * kMaxTop];  // of the warps, then of the blocks
-  uint64_t best[WARPS > 1 ? kMaxTop : 1];
-  uint2 found[WARPS][32 * kItems];  // a tile's entries that may be above the bound: value and column
+  union {
+    uint2 found[WARPS][32 * kItems];  // a tile's entries that may be above the bound: value and column
+    uint64_t list[WARPS][kMaxTop];    // at the end
+  };
   unsigned long long bound;
   RowSums warp_sums[WARPS];
   RowSums sums;
-  int count;  // entries of the list
 };
-
-// Ranks the n entries of the list; the first `top` go to sh.best in order.
-// All threads of the block.
-template <int WARPS>
-__device__ __forceinline__ void rank_list(RowShared<WARPS>& sh, int n, int top) {
-  for (int i = threadIdx.x; i < n; i += WARPS * 32) {
-    const uint64_t mine = sh.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.list[j] > mine;
-    if (rank < top) sh.best[rank] = mine;  // entries are distinct, so ranks are
+// Joins the lists of `count` warps (a power of two) two by two into warp 0's.
+template <int WARPS, int N>
+__device__ __forceinline__ void join_lists(RowShared<WARPS>& sh, TopKeys<N>& list, int count, int warp, int lane) {
+  for (int half = count / 2; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) list.store(sh.list[warp], lane);
+    __syncthreads();
+    if (warp < half) {
+      TopKeys<N> other;
+      other.load(sh.list[warp + half], lane);
+      list.join(other, lane);
+    }
   }
-  __syncthreads();
 }
 
 // N: registers a lane for the alternatives, 0 where none are asked for.
@@ -252,7 +277,8 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   constexpr int V = 16 / int(sizeof(T));  // entries of a 16-byte group
   constexpr int G = kItems / V;           // a lane's groups of a tile
   constexpr int kTile = 32 * kItems;
-  __shared__ RowShared<WARPS> sh;
+  extern __shared__ __align__(16) unsigned char row_memory[];
+  RowShared<WARPS>& sh = *reinterpret_cast<RowShared<WARPS>*>(row_memory);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / split;
   const int part = blockIdx.x % split;
@@ -302,10 +328,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   for (int n = 0; n < (N ? N : 1); ++n) list.key[n] = 0;
   uint64_t bound = 0;  // an entry has to be above this key; 0: no bound yet
   if (N && WARPS > 1) {
-    if (threadIdx.x == 0) {
-      sh.bound = 0;
-      sh.count = 0;
-    }
+    if (threadIdx.x == 0) sh.bound = 0;
     __syncthreads();
   }
   for (; tile < tiles; tile += step) {
@@ -356,11 +379,16 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
       const bool none1 = column(tile, kItems - 1) < 0 || column(tile, kItems / 2) >= a.width;
       uint32_t reached = 0;
       if (N == 1) {
+        // the maxima in order over the lanes
         uint32_t mine = none0 && none1 ? 0u : rank_bits(none1 ? half0 : none0 ? half1 : most);
-        for (int i = 0; i < a.top; ++i) {
-          reached = __reduce_max_sync(kFull, mine);
-          if (lane == __ffs(__ballot_sync(kFull, mine == reached)) - 1) mine = 0;
-        }
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+          for (int bit = size / 2; bit > 0; bit >>= 1) {
+            const uint32_t other = __shfl_xor_sync(kFull, mine, bit);
+            mine = ((lane & bit) == 0) == ((lane & size) == 0) ? max(mine, other) : min(mine, other);
+          }
+        reached = __shfl_sync(kFull, mine, a.top - 1);
       } else {
         reached = __reduce_min_sync(kFull, min(none0 ? 0u : rank_bits(half0), none1 ? 0u : rank_bits(half1)));
       }
@@ -395,7 +423,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
       for (int i = 0; i < n; ++i) list.insert(key_of(i), lane);
     } else {
 #pragma unroll 1
-      for (int i = 0; i < n; i += 32) list.merge(i + lane < n ? key_of(i + lane) : 0, lane);
+      for (int i = 0; i < n; i += 32) list.merge(i + lane < n ? key_of(i + lane) : 0, n - i, lane);
     }
     __syncwarp();
     const uint64_t last = list.at(a.top - 1);
@@ -413,39 +441,18 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     if (lane == 0) sh.warp_sums[warp] = sums;
     __syncthreads();
     sums = warp_join(lane < WARPS ? sh.warp_sums[lane % WARPS] : none, k);
-    if (N) {
-      // entries that every warp's bound leaves among the first
-      const uint64_t reached = sh.bound;
-#pragma unroll
-      for (int n = 0; n < (N ? N : 1); ++n)
-        if (n * 32 + lane < a.top && list.key[n] && list.key[n] >= reached) sh.list[atomicAdd(&sh.count, 1)] = list.key[n];
-      __syncthreads();
-      rank_list(sh, sh.count, a.top);
-    }
+    if (N) join_lists<WARPS, N ? N : 1>(sh, list, WARPS, warp, lane);
   }
   if (split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) sh.sums = sums;
+    if (N && warp == 0) list.store(sh.list[0], lane);
     cluster.sync();
-    if (part == 0) {
-      sums = warp_join(lane < split ? cluster.map_shared_rank(&sh, lane % split)->sums : none, k);
-      if (N && WARPS > 1) {
-        // a block's best are its first min(count, top)
-        const int mine = min(sh.count, a.top);
-        for (int i = threadIdx.x; i < mine; i += WARPS * 32) sh.list[i] = sh.best[i];
-        __syncthreads();
-        if (threadIdx.x == 0) sh.count = mine;
-        __syncthreads();
-        for (int i = threadIdx.x; i < (split - 1) * a.top; i += WARPS * 32) {
-          const RowShared<WARPS>* other = cluster.map_shared_rank(&sh, 1 + i / a.top);
-          if (i % a.top < other->count) sh.list[atomicAdd(&sh.count, 1)] = other->best[i % a.top];
-        }
-        __syncthreads();
-        rank_list(sh, sh.count, a.top);
-      }
-    }
+    if (part == 0) sums = warp_join(lane < split ? cluster.map_shared_rank(&sh, lane % split)->sums : none, k);
+    if (N && part == 0 && warp < split) list.load(cluster.map_shared_rank(&sh, warp)->list[0], lane);
     cluster.sync();  // the parts' shared memory is read until here
     if (part) return;
+    if (N) join_lists<WARPS, N ? N : 1>(sh, list, split, warp, lane);
   }
   const bool empty = sums.s1 == 0.f;
   const float ref = empty ? 0.f : sums.ref, logs = logf(sums.s1);
@@ -460,7 +467,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   for (int n = 0; n < (N ? N : 1); ++n) {
     const int i = n * 32 + lane;
     if (warp > 0 || i >= a.top) return;
-    const uint64_t key = WARPS > 1 ? sh.best[i] : list.key[n];
+    const uint64_t key = list.key[n];
     a.top_index[row * a.top + i] = int32_t(rank_index(key));
     a.top_logprob[row * a.top + i] = empty ? -INFINITY : fmaf(rank_value(uint32_t(key >> 32)) - ref, a.scale, -logs);
   }
@@ -475,15 +482,16 @@ int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
   const int64_t room = int64_t(sm_count()) * (32 / WARPS);
   int split = 1;
   while (WARPS == kMaxWarps && split * 2 <= std::min<int64_t>(kMaxSplit, tiles) && a.rows * split * 2 <= room) split *= 2;
-  if (split == 1) {
-    kernel<<<unsigned(a.rows), WARPS * 32, 0, s>>>(a, 1, logits);
-    FG_CUDA_TRY(cudaGetLastError());
-    return FG_OK;
-  }
   static OncePerDevice ready;
-  if (split > 8 && ready.first()) {
+  if (ready.first()) {
+    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(RowShared<WARPS>))));
     FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     ready.done();
+  }
+  if (split == 1) {
+    kernel<<<unsigned(a.rows), WARPS * 32, sizeof(RowShared<WARPS>), s>>>(a, 1, logits);
+    FG_CUDA_TRY(cudaGetLastError());
+    return FG_OK;
   }
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -492,6 +500,7 @@ int launch_logprobs(const LogProbsArgs& a, const T* logits, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(a.rows * split));
   cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = sizeof(RowShared<WARPS>);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -632,12 +641,20 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     const T* x = static_cast<const T*>(logits);
-    // Warps of a row's block: with rows enough to fill the SMs a warp alone takes
-    // a row, without a barrier; fewer rows or a wide one get more.
-    const int64_t fill = int64_t(sm_count()) * 1024;
-    if (width <= 1024 || rows * 32 >= fill) return launch_logprobs<T, 1>(a, x, s);
-    if (width <= 4096) return launch_logprobs<T, 4>(a, x, s);
-    return launch_logprobs<T, kMaxWarps>(a, x, s);
+    // Warps of a row: a warp that takes more of a row pays its first tile's
+    // alternatives less often, so no more than the SMs' 32 each (up to 0.7 of
+    // them), and no more than the row has tiles; past 16, blocks of a cluster.
+    // (2048 x 32768 fp32, 8 alternatives: 2 warps 64 us, 8 warps 81, 16 warps 104.)
+    const int64_t enough = int64_t(sm_count()) * 32 * 7 / 10;
+    int warps = 1;
+    while (warps < kMaxWarps && rows * warps < enough && width > warps * 32 * kItems) warps *= 2;
+    switch (warps) {
+      case 1: return launch_logprobs<T, 1>(a, x, s);
+      case 2: return launch_logprobs<T, 2>(a, x, s);
+      case 4: return launch_logprobs<T, 4>(a, x, s);
+      case 8: return launch_logprobs<T, 8>(a, x, s);
+      default: return launch_logprobs<T, kMaxWarps>(a, x, s);
+    }
   });
 }
 
