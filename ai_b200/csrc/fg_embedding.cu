@@ -258,13 +258,25 @@ __global__ void __launch_bounds__(kSortThreads) heads_place_kernel(const uint32_
   }
 }
 
-// Sets the bit of every row that a token met.
-__global__ void __launch_bounds__(kSortThreads) met_kernel(const uint32_t* __restrict__ keys, int64_t n, int64_t vocab,
-                                                          uint32_t* __restrict__ met) {
-  const int64_t i = int64_t(blockIdx.x) * kSortThreads + threadIdx.x;
-  if (i >= n) return;
-  const uint32_t key = keys[i];
-  if (key < vocab && (i == 0 || keys[i - 1] != key)) atomicOr(met + key / 32, 1u << key % 32);
+// Marks every row that a token met, in a byte of its own. Stores to one
+// 32-byte sector queue in L2 (131072 tokens, a quarter of them in the first
+// 32 rows: 19 us), so few blocks take many tokens each, and an id's tokens
+// first meet in a table in the block's shared memory, where all but one
+// usually stay.
+constexpr int kMarkThreads = 1024;
+constexpr int kMarkBlocks = 32;
+constexpr int kMarkTable = 8192;
+__global__ void __launch_bounds__(kMarkThreads) met_kernel(const int32_t* __restrict__ ids, int64_t n, int64_t vocab,
+                                                          int padding, uint8_t* met) {
+  __shared__ int table[kMarkTable];
+  for (int i = threadIdx.x; i < kMarkTable; i += kMarkThreads) table[i] = -1;
+  __syncthreads();
+#pragma unroll 4
+  for (int64_t i = int64_t(blockIdx.x) * kMarkThreads + threadIdx.x; i < n; i += kMarkThreads * kMarkBlocks) {
+    const int id = ids[i];
+    if (id == padding || id < 0 || id >= vocab) continue;
+    if (atomicExch(&table[id % kMarkTable], id) != id) met[id] = 1;
+  }
 }
 
 __global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* count) {
@@ -302,10 +314,11 @@ struct GroupArgs {
   uint32_t* totals;  // [kMaxBlocks, kRadix] and kMaxBlocks more
   uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
   uint32_t* pos[2];
-  uint32_t* met;     // a bit for every row, set where a token met it; null: not asked for
+  uint8_t* met;      // a byte for every row, 1 where a token met it; null: not asked for
   uint32_t* place;   // with row_ids and count: the rows met; null: not asked for
   int32_t* row_ids;
   int32_t* count;
+  uint32_t* long_runs;  // a count that starts at 0
   int* err;
 };
 
@@ -353,8 +366,11 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   const int blocks = gridDim.x, block = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t mask = (1u << a.digit) - 1;
-  if (a.met)  // the barriers of the passes come before the first bit is set
-    for (int64_t i = block * kGroupThreads + tid; i < (a.vocab + 31) / 32; i += blocks * kGroupThreads) __stcg(a.met + i, 0u);
+  let_next_start();
+  if (block == 0 && tid == 0) *a.long_runs = 0;
+  if (a.met)  // the barriers of the passes come before the first mark
+    for (int64_t i = block * kGroupThreads + tid; i < (a.vocab + 15) / 16; i += blocks * kGroupThreads)
+      __stcg(reinterpret_cast<uint4*>(a.met) + i, make_uint4(0, 0, 0, 0));
   uint2 mine[ITEMS];  // (key, position) of consecutive tokens of a warp, 32 a round
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     const uint32_t prev = i > 0 && i < a.n ? __ldcg(a.key[0] + i - 1) : 0xffffffffu;
     heads[k] = __ballot_sync(kFull, key[k] < a.vocab && prev != key[k]);
     if (lane == 0) sh.heads[k * kGroupWarps + warp] = __popc(heads[k]);
-    if (a.met && heads[k] >> lane & 1) atomicOr(a.met + key[k] / 32, 1u << key[k] % 32);
+    if (a.met && heads[k] >> lane & 1) a.met[key[k]] = 1;
   }
   if (!a.place) return;
   __syncthreads();
@@ -575,10 +591,14 @@ __device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, 
 // ------------------------------------------------------------------ sums
 // A warp sums one chunk of sorted tokens over 32·VEC columns, with kRing
 // rows in flight (4, 6 and 8 of them, with the warps that their registers
-// leave room for, measured alike). A run of one id that lies within the chunk is written as
-// its row; a run that came in from the chunk before leaves its sum in
-// head[chunk], one that goes on into the next chunk (and began here) in
-// tail[chunk].
+// leave room for, measured alike). A run of one id no longer than a chunk
+// belongs to the chunk in which it begins, wherever it ends. A longer run is
+// cut where the chunks are: the part in the chunk in which it begins
+// goes to tail[chunk], the others to head[chunk], and join_kernel adds them.
+// (Runs of any length cut at the chunks' ends: four times as many to join,
+// 23 us of 131072 frequent tokens' 240.)
+// Bytes of a dense gradient from which its zeros are written beside the sort.
+constexpr int64_t kZerosFirst = int64_t(32) << 20;
 constexpr int kMaxChunk = 32;
 constexpr int kMinChunk = 4;
 constexpr int kRing = 4;
@@ -597,10 +617,11 @@ struct SumArgs {
   int accumulate;
   float* head;
   float* tail;  // [chunks, dim] each
+  uint32_t* long_runs;  // their number, then the chunks in which they begin, in any order
   // blocks that zero the rows without tokens, spread among those that sum
   int64_t rows;
   const int32_t* count;  // rows met, of the compact gradient; null: the dense one
-  const uint32_t* met;   // a bit for every row of the dense one; null: no tokens
+  const uint8_t* met;    // a byte for every row of the dense one, 1: has tokens; null: no tokens
   int sum_blocks, zero_blocks;
 };
 
@@ -625,10 +646,12 @@ template <typename TG, int VEC>
 __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t unit, TG* grad, int lane) {
   const int64_t r0 = unit / a.slices * 32;
   const int col = (int(unit % a.slices) * 32 + lane) * VEC;
-  if (r0 >= a.rows || col >= a.dim) return;
+  if (r0 >= a.rows) return;
   const int64_t count = a.count ? int64_t(*a.count) - r0 : 0;
-  unsigned keep = a.count ? (count >= 32 ? kFull : count > 0 ? (1u << count) - 1 : 0) : a.met ? a.met[r0 / 32] : 0;
+  unsigned keep = count >= 32 ? kFull : count > 0 ? (1u << count) - 1 : 0;
+  if (!a.count && a.met) keep = __ballot_sync(kFull, r0 + lane < a.rows && a.met[r0 + lane]);
   if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
+  if (col >= a.dim) return;
   Pack<TG, VEC> z;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
@@ -636,6 +659,15 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t unit, TG* gr
 #pragma unroll 8
   for (int r = 0; r < 32; ++r)
     if (!(keep >> r & 1)) z.store(g + r * a.ldg);
+}
+
+// The zeros alone, while the tokens are sorted: needs the marks of the rows
+// met, not the sort that runs before it in the stream. Its blocks wait for the
+// sort at their end, so that what comes after it comes after both.
+template <typename TG, int VEC>
+__global__ void __launch_bounds__(kSumWarps * 32) zero_kernel(SumArgs a, TG* grad) {
+  zero_rows<TG, VEC>(a, int64_t(blockIdx.x) * kSumWarps + (threadIdx.x >> 5), grad, threadIdx.x & 31);
+  wait_for_previous();
 }
 
 template <typename TY, typename TG, int VEC>
@@ -654,41 +686,57 @@ __global__ void __launch_bounds__(kSumWarps * 32, 4) sum_kernel(SumArgs a, const
   const int64_t i0 = chunk * size;
   if (i0 >= a.n) return;
   const uint32_t key = lane < size && i0 + lane < a.n ? a.keys[i0 + lane] : 0xffffffffu;
+  const uint32_t left = i0 + lane >= 32 ? a.keys[i0 + lane - 32] : 0xffffffffu;
+  const uint32_t right = i0 + size + lane < a.n ? a.keys[i0 + size + lane] : 0xffffffffu;
   const int count = __popc(__ballot_sync(kFull, key < a.vocab));  // tokens without a row come last
   if (count == 0) return;
+  const uint32_t first_key = __shfl_sync(kFull, key, 0), last_key = __shfl_sync(kFull, key, count - 1);
+  // tokens of the first run before this chunk and in it, of the last one in it and behind it
+  const int before = __clz(~__ballot_sync(kFull, left == first_key));
+  const int first = __popc(__ballot_sync(kFull, key == first_key)), last = __popc(__ballot_sync(kFull, key == last_key));
+  const unsigned same = __ballot_sync(kFull, right == last_key);
+  const int behind = count < size ? 0 : same == kFull ? 32 : __ffs(~same) - 1;
+  const bool came = before > 0;
+  const bool long_first = before + first + (first == size ? behind : 0) > size;
+  const bool goes = behind > 0 && !(came && first == size);  // the last run began here
+  const bool long_last = goes && last + behind > size;
+  const int begin = came && !long_first ? first : 0;
+  const int end = count + (goes && !long_last ? behind : 0);
+  if (begin >= end) return;
   const uint32_t pos = lane < count ? a.pos[i0 + lane] : 0;
+  const uint32_t pos_behind = lane < end - count ? a.pos[i0 + count + lane] : 0;
   const uint32_t row = lane < count ? (a.place ? a.place[i0 + lane] : key) : 0;
-  const bool came = i0 > 0 && a.keys[i0 - 1] == __shfl_sync(kFull, key, 0);
-  const bool goes = count == size && i0 + size < a.n && a.keys[i0 + size] == __shfl_sync(kFull, key, size - 1);
   const uint32_t next = __shfl_down_sync(kFull, key, 1);
-  // the last tokens of the runs; those whose sum is only a part of the row's
-  const unsigned ends = __ballot_sync(kFull, lane == count - 1 || (lane < count && next != key));
-  const unsigned heads = came ? ends & -ends : 0, tails = goes ? (1u << (count - 1)) & ~heads : 0;
+  // the last tokens of the runs, and of the parts of long ones
+  uint64_t ends = __ballot_sync(kFull, lane < count - 1 && next != key);
+  ends |= uint64_t(1) << (end - 1);
+  const int head = came && long_first ? first - 1 : -1, tail = long_last ? end - 1 : -1;
+  if (long_last && unit % a.slices == 0 && lane == 0) a.long_runs[1 + atomicAdd(a.long_runs, 1u)] = uint32_t(chunk);
   const bool in = col < a.dim;
   const TY* y = dy + col;
   Pack<TY, VEC> v[kRing];
   auto load = [&](int u, int t) {
-    const uint32_t from = __shfl_sync(kFull, pos, t & 31);
-    if (t < count && in) v[u].load(y + int64_t(from) * a.ldy);
+    const uint32_t here = __shfl_sync(kFull, pos, t & 31), there = __shfl_sync(kFull, pos_behind, (t - count) & 31);
+    if (t < end && in) v[u].load(y + int64_t(t < count ? here : there) * a.ldy);
   };
 #pragma unroll
-  for (int u = 0; u < kRing; ++u) load(u, u);
+  for (int u = 0; u < kRing; ++u) load(u, begin + u);
   float acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-  for (int t0 = 0; t0 < count; t0 += kRing) {
+  for (int t0 = begin; t0 < end; t0 += kRing) {
 #pragma unroll
     for (int u = 0; u < kRing; ++u) {
       const int t = t0 + u;
-      if (t >= count) break;
+      if (t >= end) break;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
       load(u, t + kRing);
       if (!(ends >> t & 1)) continue;
-      const uint32_t to = __shfl_sync(kFull, row, t);
+      const uint32_t to = __shfl_sync(kFull, row, min(t, count - 1));
       if (in) {
-        if ((heads | tails) >> t & 1) {
-          float* ws = (heads >> t & 1 ? a.head : a.tail) + chunk * a.dim + col;
+        if (t == head || t == tail) {
+          float* ws = (t == head ? a.head : a.tail) + chunk * a.dim + col;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) ws[i] = acc[i];
         } else {
@@ -701,27 +749,25 @@ __global__ void __launch_bounds__(kSumWarps * 32, 4) sum_kernel(SumArgs a, const
   }
 }
 
-// The runs that cross chunks: the chunk in which one begins adds the heads
-// of the chunks after it, in their order, and writes the row. A warp joins a
-// run of a few chunks; a long one (a frequent token) is shared by the block's
-// warps, which take equal consecutive parts of it. A block's warps have
-// different chunks of the same columns, so the columns of a long run meet in
-// different blocks.
+// The long runs: the part in the chunk in which one begins, and the heads of
+// the chunks after it, in their order, are its row. A warp joins a run of a
+// few chunks; one of many (a frequent token) is shared by the block's warps,
+// which take equal consecutive parts of it. A block's warps have different
+// runs and the same columns, so the columns of a run meet in different blocks.
 constexpr int kLongRun = 16;  // chunks after the first
 
 template <typename TG, int VEC>
 __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* grad) {
   __shared__ int long_run[kSumWarps];
+  __shared__ int64_t long_chunk[kSumWarps];
   __shared__ float part[kSumWarps][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int size = a.chunk;
-  const int64_t chunks = (a.n + size - 1) / size;
-  const int64_t blocks = (chunks + kSumWarps - 1) / kSumWarps;  // of a slice
-  const int64_t chunk0 = blockIdx.x % blocks * kSumWarps;
-  const int col = (int(blockIdx.x / blocks) * 32 + lane) * VEC;
-  const bool in = col < a.dim;
   wait_for_previous();
-  // sum of heads [c, c + count) in order, eight in flight
+  const int size = a.chunk, runs = int(a.long_runs[0]);
+  const int groups = (runs + kSumWarps - 1) / kSumWarps;  // of a slice
+  int col = 0;
+  bool in = false;
+  // sum of heads [c, c + count) in order, kAhead in flight
   auto add_heads = [&](float (&acc)[VEC], int64_t c, int count) {
     if (!in) return;
     for (int i = 0; i < count; i += kAhead) {
@@ -737,54 +783,71 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
     }
   };
   auto finish = [&](const float (&acc)[VEC], int64_t chunk) {
-    const int64_t last = chunk * size + size - 1;
+    const int64_t last = (chunk + 1) * size - 1;
     const int64_t row = a.place ? a.place[last] : a.keys[last];
     if (in) write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
   };
 
-  const int64_t chunk = chunk0 + warp, i0 = chunk * size, end = i0 + size;
-  int run = 0;  // chunks after this one that the run which leaves it covers
-  if (end < a.n) {
-    // the places asked for in one go: the chunk's ends, the next 32 chunks' starts
-    const int64_t start = end + int64_t(lane) * size;
-    const uint32_t key = a.keys[end - 1], first = a.keys[i0], left = i0 > 0 ? a.keys[i0 - 1] : 0xffffffffu;
-    const unsigned same = __ballot_sync(kFull, start < a.n && a.keys[start] == key);
-    if (key < a.vocab && (same & 1) && !(first == key && left == key)) {
-      run = same == kFull ? int((first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane) + size - 1) / size) : __ffs(~same) - 1;
+  for (int g = blockIdx.x; g < groups * a.slices; g += gridDim.x) {
+    const int at = warp * groups + g % groups;  // neighbours in the list, often the longest, apart
+    col = (g / groups * 32 + lane) * VEC;
+    in = col < a.dim;
+    const int64_t chunk = at < runs ? a.long_runs[1 + at] : 0, end = (chunk + 1) * size;
+    int run = 0;  // chunks after this one that the run covers
+    if (at < runs) {
+      const uint32_t key = a.keys[end - 1];
+      // the starts of the next 32 chunks, then of 32 groups of 32, or all
+      const int64_t start = end + int64_t(lane) * size, far = start + int64_t(lane) * 31 * size;
+      const unsigned same = __ballot_sync(kFull, start < a.n && a.keys[start] == key);
+      run = __ffs(~same) - 1;
+      if (same == kFull) {
+        const unsigned fars = __ballot_sync(kFull, far < a.n && a.keys[far] == key);
+        if (fars == kFull) {
+          run = int((first_token(a.keys + end, a.n - end, int64_t(key) + 1, lane) + size - 1) / size);
+        } else {
+          const int before = (__ffs(~fars) - 2) * 32;
+          const int64_t fine = start + int64_t(before) * size;
+          run = before + __popc(__ballot_sync(kFull, fine < a.n && a.keys[fine] == key));
+        }
+      }
     }
-  }
-  float acc[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  if (run > 0 && run <= kLongRun) {
-    if (in)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] = a.tail[chunk * a.dim + col + j];
-    add_heads(acc, chunk + 1, run);
-    finish(acc, chunk);
-  }
-  if (lane == 0) long_run[warp] = run > kLongRun ? run : 0;
-  __syncthreads();
-  for (int w = 0; w < kSumWarps; ++w) {
-    const int count = long_run[w];
-    if (count == 0) continue;
-    const int share = (count + kSumWarps - 1) / kSumWarps, first = warp * share;
+    float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    add_heads(acc, chunk0 + w + 1 + first, max(0, min(share, count - first)));
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) part[warp][lane * VEC + j] = acc[j];
-    __syncthreads();
-    if (warp == w) {
+    if (run > 0 && run <= kLongRun) {
       if (in)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = a.tail[chunk * a.dim + col + j];
-      for (int p = 0; p < kSumWarps; ++p)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += part[p][lane * VEC + j];
+      add_heads(acc, chunk + 1, run);
       finish(acc, chunk);
     }
+    if (lane == 0) {
+      long_run[warp] = run > kLongRun ? run : 0;
+      long_chunk[warp] = chunk;
+    }
     __syncthreads();
+    for (int w = 0; w < kSumWarps; ++w) {
+      const int count = long_run[w];
+      if (count == 0) continue;
+      const int share = (count + kSumWarps - 1) / kSumWarps, first = warp * share;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+      add_heads(acc, long_chunk[w] + 1 + first, max(0, min(share, count - first)));
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) part[warp][lane * VEC + j] = acc[j];
+      __syncthreads();
+      if (warp == w) {
+        if (in)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] = a.tail[chunk * a.dim + col + j];
+        for (int p = 0; p < kSumWarps; ++p)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += part[p][lane * VEC + j];
+        finish(acc, chunk);
+      }
+      __syncthreads();
+    }
+    __syncthreads();  // long_run is read until here
   }
 }
 
@@ -822,14 +885,14 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   int chunk = kMaxChunk;
   while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
-  const bool bits_of_rows = !compact && !accumulate && n > 0;
-  const size_t met_bytes = bits_of_rows ? round256(size_t(blocks_of(vocab, 32)) * 4) : 0;
+  const bool marks = !compact && !accumulate && n > 0;
+  const size_t met_bytes = marks ? round256(size_t(vocab)) : 0;
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
   const bool grouped_here = n <= kMaxGroup;
   const size_t hist = grouped_here ? round256((kMaxBlocks * kRadix + kMaxBlocks) * 4)
                                    : round256(size_t(tiles) * (size_t(1) << digit) * 4);
   Scratch ws(s);
-  FG_TRY(scratch_alloc(&ws.p, 5 * list + hist + 2 * part + met_bytes, s));
+  FG_TRY(scratch_alloc(&ws.p, 6 * list + hist + 2 * part + met_bytes, s));
   unsigned char* at = static_cast<unsigned char*>(ws.p);
   auto take = [&](size_t bytes) {
     void* r = at;
@@ -839,17 +902,28 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   uint32_t* key[2] = {static_cast<uint32_t*>(take(list)), static_cast<uint32_t*>(take(list))};
   uint32_t* pos[2] = {static_cast<uint32_t*>(take(list)), static_cast<uint32_t*>(take(list))};
   uint32_t* place = static_cast<uint32_t*>(take(list));
+  uint32_t* long_runs = static_cast<uint32_t*>(take(list));  // at most one in kMinChunk + 1 tokens begins one
   uint32_t* counts = static_cast<uint32_t*>(take(hist));
-  uint32_t* met = bits_of_rows ? static_cast<uint32_t*>(take(met_bytes)) : nullptr;
+  uint8_t* met = marks ? static_cast<uint8_t*>(take(met_bytes)) : nullptr;
   SumArgs a{};
   a.met = met;
+  a.long_runs = long_runs;
   a.head = static_cast<float*>(take(part));
   a.tail = static_cast<float*>(take(part));
+  // A large dense gradient's zeros are written while a cluster sorts (16 of the
+  // SMs); the rows met are then marked beforehand.
+  const bool zeros_first = met && grouped_here && n > 4 * kGroupThreads && vocab * dim * dtype_size(grad_dtype) >= kZerosFirst;
+  if (zeros_first || (met && !grouped_here)) {
+    FG_CUDA_TRY(cudaMemsetAsync(met, 0, met_bytes, s));
+    met_kernel<<<kMarkBlocks, kMarkThreads, 0, s>>>(ids, n, vocab, padding, met);
+    FG_CUDA_TRY(cudaGetLastError());
+  }
   if (n > 0 && grouped_here) {
-    GroupArgs g{ids, int(n), vocab, padding, passes, digit, counts, {key[0], key[1]}, {pos[0], pos[1]}, met,
-                compact ? place : nullptr, row_ids, count, err};
+    GroupArgs g{ids, int(n), vocab, padding, passes, digit, counts, {key[0], key[1]}, {pos[0], pos[1]}, zeros_first ? nullptr : met,
+                compact ? place : nullptr, row_ids, count, long_runs, err};
     FG_TRY(group_tokens(g, s));
   } else if (n > 0) {
+    FG_CUDA_TRY(cudaMemsetAsync(long_runs, 0, sizeof(uint32_t), s));
     for (int p = 0; p < passes; ++p) {
       const uint32_t* k = p ? key[(p + 1) & 1] : nullptr;
       sort_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, n, vocab, padding, p * digit, digit, counts, err);
@@ -867,10 +941,6 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.ldg = ldg;
   a.scale = scale;
   a.accumulate = accumulate;
-  if (met && !grouped_here) {
-    FG_CUDA_TRY(cudaMemsetAsync(met, 0, met_bytes, s));
-    met_kernel<<<unsigned(blocks_of(n, kSortThreads)), kSortThreads, 0, s>>>(a.keys, n, vocab, met);
-  }
   if (compact) a.place = place;
   if (compact && !grouped_here) {
     heads_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(a.keys, n, vocab, counts);
@@ -884,22 +954,26 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.rows = compact ? n : vocab;
   a.count = count;
   const int64_t sum_blocks = blocks_of(chunks * a.slices, kSumWarps);
-  const int64_t zero_blocks = accumulate ? 0 : blocks_of(blocks_of(a.rows, 32) * slices, kSumWarps);
+  const int64_t all_zero_blocks = accumulate ? 0 : blocks_of(blocks_of(a.rows, 32) * slices, kSumWarps);
+  const int64_t zero_blocks = zeros_first ? 0 : all_zero_blocks;
   if (sum_blocks + zero_blocks > INT32_MAX) return set_error(FG_EINVAL, "embedding gradient: too many tokens times columns");
   if (sum_blocks + zero_blocks == 0) return FG_OK;
   a.sum_blocks = int(sum_blocks);
   a.zero_blocks = int(zero_blocks);
   const unsigned threads = kSumWarps * 32, blocks = unsigned(sum_blocks + zero_blocks);
-  const unsigned join_blocks = unsigned(blocks_of(chunks, kSumWarps) * a.slices);
+  // as many blocks as there may be long runs, up to two rounds of the SMs' blocks
+  const unsigned join_blocks = unsigned(std::min<int64_t>(blocks_of(n / (chunk + 1), kSumWarps) * a.slices, int64_t(sm_count()) * 6));
   return by_dtype(grad_dtype, [&](auto tg) {
     using TG = typename decltype(tg)::type;
     TG* g = static_cast<TG*>(grad);
+    if (zeros_first)
+      FG_TRY(launch_after(wide ? zero_kernel<TG, 4> : zero_kernel<TG, 1>, unsigned(all_zero_blocks), threads, s, a, g));
     FG_TRY(by_dtype(dy_dtype, [&](auto ty) {
       using TY = typename decltype(ty)::type;
       return launch_after(wide ? sum_kernel<TY, TG, 4> : sum_kernel<TY, TG, 1>, blocks, threads, s, a,
                           static_cast<const TY*>(dy), g);
     }));
-    if (n <= chunk) return FG_OK;  // one chunk: nothing crosses
+    if (n <= chunk) return FG_OK;
     return launch_after(wide ? join_kernel<TG, 4> : join_kernel<TG, 1>, join_blocks, threads, s, a, g);
   });
 }

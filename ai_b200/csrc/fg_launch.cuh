@@ -12,6 +12,10 @@ namespace fg {
 
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The next kernel in the stream, where it was launched with launch_after, may
+// be set up once all blocks of this one have come here.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <typename... P, typename... A>
 int launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t s, const A&... args) {
   cudaLaunchAttribute attr{};
