@@ -572,7 +572,9 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(LogProbsGra
     Pack<T, V> out;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float lp = fmaf(in[g].get(i), a.scale, -lse);
+      // the product rounded as it is in lse, so that the largest entry of a row
+      // that has all the probability has exactly 1
+      const float lp = __fsub_rn(__fmul_rn(in[g].get(i), a.scale), lse);
       const float p = ex2_approx(lp * kLog2e);
       float d = g0 * ((j + i == t ? 1.f : 0.f) - p);
       if (ENTROPY && p != 0.f) d = fmaf(-h * p, lp + H, d);
