@@ -762,3 +762,100 @@ def test_refusals(cuda):
     for call in bad:
         with pytest.raises(train.TensorError):
             call()
+
+
+# ------------------------------------------- every way the work is divided
+@pytest.mark.parametrize("n,vocab,dim", [(40000, 3, 8), (100000, 2, 4), (70000, 1000, 40), (270000, 1000, 12), (265000, 30000, 5)])
+def test_grad_long_runs(cuda, n, vocab, dim):
+    """Runs of thousands of chunks, more tokens than one cluster sorts, and
+    the rows no token met among them."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n)
+    dy = _randn((n, dim), g, cuda)
+    ids = torch.randint(0, max(1, vocab - 1), (n,), generator=g, device=cuda, dtype=torch.int32)
+    ids[n // 3:2 * n // 3] = 1
+    want, err = _grad_want(dy, ids, vocab, 1.0, -1)
+    got = train.EmbeddingGrad(dy, ids, vocab)
+    _near(got, want, err)
+    assert torch.equal(got, train.EmbeddingGrad(dy, ids, vocab))
+    _check_rows(train.EmbeddingGradRows(dy, ids, vocab), want, err, ids, -1)
+    old = torch.ones(vocab, dim, device=cuda)
+    new = train.EmbeddingGrad(dy, ids, vocab, out=old.clone(), accumulate=True)
+    _near(new, want + 1, err + u * (want.abs() + (want + 1).abs()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5000, 20001])
+def test_grad_of_a_large_table(cuda, dtype, n):
+    """Zeros written beside the sort: 262144 rows, few of them met."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n)
+    vocab, dim = 262144, 96
+    dy = _randn((n, dim), g, cuda, dtype)
+    ids = (vocab ** torch.rand(n, generator=g, device=cuda, dtype=torch.float64)).int().clamp(0, vocab - 1)
+    ids[::50] = vocab - 1
+    ids[::77] = -1
+    want, err = _grad_want(dy, ids, vocab, 0.5, -1)
+    out = torch.full((vocab, dim), 3.0, device=cuda, dtype=_dt(dtype))
+    got = train.EmbeddingGrad(dy, ids, vocab, scale=0.5, out=out)
+    _near(got, want, err)
+    still = want.abs().sum(1) == 0
+    assert not got[still].any()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width,top", [(4000, 1537, 9), (2000, 1100, 33), (900, 2100, 5), (450, 4200, 64), (240, 9000, 20),
+                                            (100, 40000, 20), (40, 100001, 64), (9000, 30, 30), (5000, 513, 0)])
+def test_logprobs_divisions(cuda, dtype, rows, width, top):
+    """One to sixteen warps a row, one to sixteen blocks."""
+    import torch
+
+    g = _gen(cuda, rows)
+    x = _randn((rows, width), g, cuda, dtype) * 2
+    t = torch.randint(-1, width, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    _check_logprobs(x, t, 3.0, top)
+
+
+def test_operators_in_a_graph(cuda):
+    """Captured once, replayed on new contents of the same tensors."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 4)
+    table = _randn((3000, 128), g, cuda)
+    ids = torch.randint(0, 3000, (6000,), generator=g, device=cuda, dtype=torch.int32)
+    logits = _randn((64, 5000), g, cuda)
+    t = torch.randint(0, 5000, (64,), generator=g, device=cuda, dtype=torch.int32)
+    one = torch.ones(64, device=cuda)
+
+    def all_of_them():
+        y = train.Embedding(table, ids, scale=2.0)
+        dense = train.EmbeddingGrad(y, ids, 3000)
+        rows = train.EmbeddingGradRows(y, ids, 3000)
+        p = train.LogProbs(logits, t, top=5)
+        d = train.LogProbsGrad(logits, t, p.LogSum, one)
+        norm = train.ClipGradNorm([dense, rows.Rows, d], 1.0)
+        return [y, dense, *rows, *p, d, norm]
+
+    side = torch.cuda.Stream(cuda)
+    with torch.cuda.stream(side):
+        all_of_them()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = all_of_them()
+    for _ in range(2):
+        ids.copy_(torch.randint(0, 3000, (6000,), generator=g, device=cuda, dtype=torch.int32))
+        logits.copy_(_randn((64, 5000), g, cuda))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, all_of_them()):
+            assert torch.equal(a, b)
