@@ -94,6 +94,11 @@ struct Pack {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) reinterpret_cast<Part*>(p)[i] = part[i];
   }
+  // not to be read again soon
+  __device__ __forceinline__ void store_past(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) __stcs(reinterpret_cast<Part*>(p) + i, part[i]);
+  }
   __device__ __forceinline__ float get(int i) const { return widen(v[i]); }
   __device__ __forceinline__ void set(int i, float x) { v[i] = narrow<T>(x); }
 };

@@ -166,12 +166,11 @@ def EmbeddingGradRows(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: fl
     synchronisation: room for as many rows as there are tokens."""
     op = "EmbeddingGradRows"
     code, dy, ld, ids, n, dim, index = _grad_args(op, dy, ids, vocab, dtype)
-    row_ids = ids.new_empty(n + 1)
+    row_ids, count = ids.new_empty(n), ids.new_empty(1)
     rows = dy.new_empty((n, dim), dtype=dtype)
-    at = row_ids.data_ptr()
-    _run("fg_embedding_grad_rows", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding, at,
-         rows.data_ptr(), _DTYPES[rows.dtype], dim, at + 4 * n)
-    return RowsGrad(row_ids[:n], rows, row_ids[n:])
+    _run("fg_embedding_grad_rows", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding,
+         row_ids.data_ptr(), rows.data_ptr(), _DTYPES[rows.dtype], dim, count.data_ptr())
+    return RowsGrad(row_ids, rows, count)
 
 
 class LogProbsResult(NamedTuple):
