@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
       Pack<float, VEC> h[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (i + u < count) h[u].load(a.head + (c + i + u) * a.dim + col);
+        if (i + u < count) h[u].load_own(a.head + (c + i + u) * a.dim + col);  // written while this kernel waited
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
         if (i + u < count)

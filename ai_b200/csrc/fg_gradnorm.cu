@@ -166,12 +166,12 @@ __global__ void __launch_bounds__(kNormThreads, 8) squares_kernel(const __grid_c
 
 template <int N>
 __global__ void __launch_bounds__(kNormThreads, 4) clip_kernel(const __grid_constant__ TensorList<N> t,
-                                                           const double* __restrict__ partial, int partials,
+                                                           const double* partial, int partials,
                                                            float max_norm, float* norm) {
   __shared__ double shared[kNormThreads / 32];
   wait_for_previous();
   double s = 0;
-  for (int i = threadIdx.x; i < partials; i += kNormThreads) s += partial[i];
+  for (int i = threadIdx.x; i < partials; i += kNormThreads) s += __ldcg(partial + i);
   const double total = sqrt(block_sum(s, shared));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = float(total);
   const bool clips = total > double(max_norm) && isfinite(total);

@@ -1,7 +1,8 @@
 // Launching a kernel so that it overlaps the end of the one before it in its
 // stream (programmatic dependent launch): its blocks may be set up while the
 // last blocks of that one still run. They call wait_for_previous() before
-// anything that it wrote, or reads, is touched.
+// anything that it wrote, or reads, is touched; and what it wrote is not read
+// through the read-only path (__ldg), for it changes in the kernel's lifetime.
 #pragma once
 
 #include <cuda_runtime.h>
