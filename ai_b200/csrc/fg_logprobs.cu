@@ -163,6 +163,7 @@ __device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
 // by two, in the block and then by the cluster's first block.
 constexpr int kItems = 16;
 constexpr int kMany = 24;      // lanes with entries above the bound that ask for another bound first
+constexpr uint32_t kAnyColumn = 0x7fffffffu;  // of a bound that is a value only: behind all columns
 constexpr int kFew = 3;        // entries that are put in their places one by one
 constexpr int kMaxSplit = 16;  // blocks of a cluster
 constexpr int kMaxWarps = 16;  // of a block
@@ -327,6 +328,16 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
 #pragma unroll
   for (int n = 0; n < (N ? N : 1); ++n) list.key[n] = 0;
   uint64_t bound = 0;  // an entry has to be above this key; 0: no bound yet
+  // the least value above the bound: the bound's own for columns before its
+  // own, the next one for columns behind it
+  float least_before = NAN, least_behind = NAN;
+  uint32_t bound_column = 0;
+  auto raise = [&](uint64_t to) {
+    bound = to;
+    bound_column = rank_index(to);
+    least_before = rank_value(uint32_t(to >> 32));
+    least_behind = rank_value(uint32_t(to >> 32) + 1);
+  };
   if (N && WARPS > 1) {
     if (threadIdx.x == 0) sh.bound = 0;
     __syncthreads();
@@ -364,13 +375,12 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     add_kept(sums.s2, lost2, s2.x + s2.y);
     if (N == 0) continue;
 
-    if (WARPS > 1) bound = larger(bound, *static_cast<volatile unsigned long long*>(&sh.bound));
-    // the least value that may be above the bound: its own value is not when
-    // its column comes before the tile's
-    auto least_value = [&]() {
-      return bound ? rank_value(uint32_t(bound >> 32) + (int64_t(rank_index(bound)) < column(tile, 0) - lane * V)) : NAN;
-    };
-    float least = least_value();
+    float least = least_behind;
+    if (WARPS > 1) {
+      const uint64_t told = *static_cast<volatile unsigned long long*>(&sh.bound);
+      if (told > bound) raise(told);
+      least = column(tile, 0) - lane * V > int(bound_column) ? least_behind : least_before;
+    }
     const unsigned lanes = __ballot_sync(kFull, !(most < least));
     if (lanes == 0) continue;
     if (bound == 0 || __popc(lanes) > kMany) {
@@ -392,10 +402,10 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
       } else {
         reached = __reduce_min_sync(kFull, min(none0 ? 0u : rank_bits(half0), none1 ? 0u : rank_bits(half1)));
       }
-      if (uint64_t(reached) << 32 > bound) {
-        bound = uint64_t(reached) << 32;
+      if (reached && uint64_t(reached) << 32 > bound) {
+        raise(uint64_t(reached) << 32 | (0xffffffffu - kAnyColumn));
         if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
-        least = least_value();
+        least = least_before;
       }
     }
     uint2* found = sh.found[warp];
@@ -428,7 +438,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     __syncwarp();
     const uint64_t last = list.at(a.top - 1);
     if (last > bound) {
-      bound = last;
+      raise(last);
       if (WARPS > 1 && lane == 0) atomicMax(&sh.bound, bound);
     }
   }
