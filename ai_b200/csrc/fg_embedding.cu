@@ -310,8 +310,8 @@ struct GroupArgs {
   const int32_t* ids;
   int n;
   int64_t vocab;
-  int padding, passes, digit;
-  uint32_t* totals;  // [kMaxBlocks, kRadix] and kMaxBlocks more
+  int padding, passes;
+  uint32_t* totals;  // [kMaxBlocks, kWords], two 16-bit totals each, and kMaxBlocks more
   uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
   uint32_t* pos[2];
   uint8_t* met;      // a byte for every row, 1 where a token met it; null: not asked for
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = gridDim.x, block = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t mask = (1u << a.digit) - 1;
+  constexpr uint32_t mask = kRadix - 1;
   let_next_start();
   if (block == 0 && tid == 0) *a.long_runs = 0;
   if (a.met)  // the barriers of the passes come before the first mark
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   for (int k = 0; k < ITEMS; ++k)  // places past the last token sort behind every key
     mine[k].x = int(mine[k].y) < a.n ? token_key(int(mine[k].x), a.vocab, a.padding, a.err) : 0xffffffffu;
   for (int p = 0; p < a.passes; ++p) {
-    const int shift = p * a.digit;
+    const int shift = p * kMaxDigit;
     uint32_t* key_to = a.key[(a.passes - 1 - p) & 1];
     uint32_t* pos_to = a.pos[(a.passes - 1 - p) & 1];
     if (p > 0) {
@@ -397,18 +397,22 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     for (int i = 0; i < kGroupWarps * kWords / 4; i += kGroupThreads) zero[i + tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     uint16_t* count = reinterpret_cast<uint16_t*>(sh.counter[warp]);
+    // the lanes of each token's digit, for all rounds before the first is counted
     uint32_t rank[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & mask;
-      unsigned same = kFull;
+      const uint32_t d = mine[k].x >> shift;
+      uint32_t differ = 0;
 #pragma unroll
       for (int b = 0; b < kMaxDigit; ++b) {
-        if (b == a.digit) break;
         const bool set = d >> b & 1;
-        const unsigned vote = __ballot_sync(kFull, set);
-        same &= set ? vote : ~vote;
+        differ |= __ballot_sync(kFull, set) ^ (set ? kFull : 0u);
       }
+      rank[k] = ~differ;
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1), same = rank[k];
       const uint32_t before = __popc(same & ((1u << lane) - 1)), seen = count[d];
       rank[k] = seen + before;
       __syncwarp();
@@ -429,21 +433,23 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
       sh.offset[half][word] = run;
     }
     __syncthreads();
-    // this thread's digit: its total, and where it starts in the block's order
-    uint32_t total = 0;
-    {
-      uint16_t* offset = reinterpret_cast<uint16_t*>(sh.offset);
+    // a word's two digits: their totals, and where they start in the block's order
+    uint32_t pair = 0, start = 0;
+    if (tid < kWords) {
 #pragma unroll
       for (int h = 0; h < kHalf; ++h) {
-        const uint32_t c = offset[h * kRadix + tid];
-        offset[h * kRadix + tid] = uint16_t(total);
-        total += c;
+        const uint32_t c = sh.offset[h][tid];
+        sh.offset[h][tid] = pair;
+        pair += c;
       }
+      __stcg(a.totals + block * kWords + tid, pair);
     }
-    __stcg(a.totals + block * kRadix + tid, total);
     uint32_t sum;
-    const uint32_t start = block_scan(total, sh.warp_sum, &sum);
-    sh.start[tid] = start;
+    start = block_scan((pair & 0xffffu) + (pair >> 16), sh.warp_sum, &sum);
+    if (tid < kWords) {
+      sh.start[2 * tid] = start;
+      sh.start[2 * tid + 1] = start + (pair & 0xffffu);
+    }
     __syncthreads();
     const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset[warp / kHalfWarps]);
 #pragma unroll
@@ -455,15 +461,21 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) sh.local[rank[k]] = mine[k];
     cluster.sync();
-    uint32_t of[kMaxBlocks], all = 0, before = 0;
+    uint32_t of[kMaxBlocks], low = 0, high = 0, low_before = 0, high_before = 0;
 #pragma unroll
-    for (int b = 0; b < kMaxBlocks; ++b) of[b] = b < blocks ? __ldcg(a.totals + b * kRadix + tid) : 0;
+    for (int b = 0; b < kMaxBlocks; ++b) of[b] = b < blocks && tid < kWords ? __ldcg(a.totals + b * kWords + tid) : 0;
 #pragma unroll
     for (int b = 0; b < kMaxBlocks; ++b) {
-      all += of[b];
-      before += b < block ? of[b] : 0;
+      low += of[b] & 0xffffu;
+      high += of[b] >> 16;
+      low_before += b < block ? of[b] & 0xffffu : 0;
+      high_before += b < block ? of[b] >> 16 : 0;
     }
-    sh.base[tid] = block_scan(all, sh.warp_sum, &sum) + before - start;
+    const uint32_t first = block_scan(low + high, sh.warp_sum, &sum);
+    if (tid < kWords) {
+      sh.base[2 * tid] = first + low_before - start;
+      sh.base[2 * tid + 1] = first + low + high_before - (start + (pair & 0xffffu));
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
@@ -475,16 +487,21 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
         __stcg(pos_to + to, it.y);
       }
     }
+    if (p + 1 == a.passes && !a.met && !a.place) return;
     cluster.sync();
   }
   // where the rows begin
   unsigned heads[ITEMS];
-  uint32_t key[ITEMS];
+  uint32_t key[ITEMS], left[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int i = block * kPart + k * kGroupThreads + tid;
     key[k] = i < a.n ? __ldcg(a.key[0] + i) : 0xffffffffu;
-    const uint32_t prev = i > 0 && i < a.n ? __ldcg(a.key[0] + i - 1) : 0xffffffffu;
+    left[k] = lane == 0 && i > 0 && i < a.n ? __ldcg(a.key[0] + i - 1) : 0xffffffffu;
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t lower = __shfl_up_sync(kFull, key[k], 1), prev = lane == 0 ? left[k] : lower;
     heads[k] = __ballot_sync(kFull, key[k] < a.vocab && prev != key[k]);
     if (lane == 0) sh.heads[k * kGroupWarps + warp] = __popc(heads[k]);
     if (a.met && heads[k] >> lane & 1) a.met[key[k]] = 1;
@@ -496,14 +513,11 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   uint32_t block_heads;
   const uint32_t heads_before = block_scan(counts ? sh.heads[tid % (kGroupWarps * ITEMS)] : 0, sh.warp_sum, &block_heads);
   if (counts) sh.heads[tid] = heads_before;
-  if (tid == 0) __stcg(a.totals + kMaxBlocks * kRadix + block, block_heads);
+  if (tid == 0) __stcg(a.totals + kMaxBlocks * kWords + block, block_heads);
   cluster.sync();
-  uint32_t before = 0, total = 0;
-  for (int b = 0; b < blocks; ++b) {
-    const uint32_t c = __ldcg(a.totals + kMaxBlocks * kRadix + b);
-    total += c;
-    if (b < block) before += c;
-  }
+  // a lane for every block's count
+  const uint32_t of_block = lane < blocks ? __ldcg(a.totals + kMaxBlocks * kWords + lane) : 0;
+  const uint32_t total = __reduce_add_sync(kFull, of_block), before = __reduce_add_sync(kFull, lane < block ? of_block : 0);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int i = block * kPart + k * kGroupThreads + tid;
@@ -962,7 +976,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   const size_t met_bytes = marks ? round256(size_t(vocab)) : 0;
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
   const bool grouped_here = n <= kMaxGroup;
-  const size_t hist = grouped_here ? round256((kMaxBlocks * kRadix + kMaxBlocks) * 4)
+  const size_t hist = grouped_here ? round256((kMaxBlocks * kWords + kMaxBlocks) * 4)
                                    : round256(size_t(tiles) * (size_t(1) << digit) * 4);
   Scratch ws(s);
   FG_TRY(scratch_alloc(&ws.p, 6 * list + hist + 2 * part + met_bytes, s));
@@ -992,7 +1006,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     FG_CUDA_TRY(cudaGetLastError());
   }
   if (n > 0 && grouped_here) {
-    GroupArgs g{ids, int(n), vocab, padding, passes, digit, counts, {key[0], key[1]}, {pos[0], pos[1]}, zeros_first ? nullptr : met,
+    GroupArgs g{ids, int(n), vocab, padding, passes, counts, {key[0], key[1]}, {pos[0], pos[1]}, zeros_first ? nullptr : met,
                 compact ? place : nullptr, row_ids, count, long_runs, err};
     FG_TRY(group_tokens(g, s));
   } else if (n > 0) {

@@ -18,6 +18,7 @@ is skipped, and reported by ``Check``. Shape and type errors raise
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -25,6 +26,7 @@ import torch
 from . import _lib
 from .tensor import TensorError, _fail
 
+_TYPE_OF = attrgetter("dtype")
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
@@ -261,23 +263,26 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
     n = len(grads)
     if n == 0:
         _fail(op, "no gradients")
+    # one pass of C calls for each thing asked of the tensors: there may be hundreds
+    T = torch.Tensor
     try:
-        codes = [_DTYPES[g.dtype] for g in grads]
+        types = list(map(_TYPE_OF, grads))
+        codes = list(map(_DTYPES.__getitem__, types))
         index = grads[0].get_device()
-        alike = index >= 0 and all([g.get_device() == index and g.is_contiguous() for g in grads])
-    except (KeyError, AttributeError):
+        alike = index >= 0 and set(map(T.get_device, grads)) == {index} and all(map(T.is_contiguous, grads))
+        sizes = list(map(T.numel, grads))
+    except (KeyError, AttributeError, TypeError):
         _fail(op, "gradients must be float32, bfloat16 or float16 tensors")
     if not alike:
         _fail(op, "gradients must be contiguous tensors on one CUDA device")
-    sizes = [g.numel() for g in grads]
     outs = outs_at = None
     if out is not None:
-        if len(out) != n or not all([o.dtype == g.dtype and o.numel() == size and o.get_device() == index and
-                                     o.is_contiguous() for o, g, size in zip(out, grads, sizes)]):
+        if len(out) != n or list(map(_TYPE_OF, out)) != types or list(map(T.numel, out)) != sizes or \
+                set(map(T.get_device, out)) != {index} or not all(map(T.is_contiguous, out)):
             _fail(op, "out must match the gradients' sizes, types and device, contiguous")
-        outs = array("Q", [o.data_ptr() for o in out])
+        outs = array("Q", map(T.data_ptr, out))
         outs_at = outs.buffer_info()[0]
-    ins, sizes, codes = array("Q", [g.data_ptr() for g in grads]), array("q", sizes), array("i", codes)
+    ins, sizes, codes = array("Q", map(T.data_ptr, grads)), array("q", sizes), array("i", codes)
     norm = grads[0].new_empty((), dtype=torch.float32)
     _run("fg_clip_grad_norm", index, n, ins.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], outs_at,
          max_norm, norm.data_ptr())
