@@ -5,12 +5,18 @@
 //   lookup:   y[t] = scale · W[id_t]
 //   gradient: G[v] = scale · Σ_{t : id_t = v} dy[t]
 //
-// The gradient sorts the tokens by id (a stable radix sort, so a row's
-// tokens stay in their order), cuts the sorted tokens into chunks of equal
-// length however often a token occurs, sums each chunk's runs of one id in
-// registers and joins the runs that cross chunks in a second kernel. Sums
-// are in 32 bits in an order that depends on the ids alone, so a repeated
-// call gives the same bits; a sum is rounded once, when its row is written.
+// The gradient sorts the tokens by id, stably, so a row's tokens stay in
+// their order (by counting up to 2048 tokens, within one cluster up to 262144,
+// through memory beyond); cuts the sorted tokens into chunks of equal length
+// however often a token occurs; sums the runs of one id in registers; and
+// joins the runs that are longer than a chunk in a second kernel. Sums are in
+// 32 bits in an order that depends on the ids alone, so a repeated call gives
+// the same bits; a sum is rounded once, when its row is written.
+//
+// Bound by memory for many tokens: 131072 of 768 fp32 into a table of 262144
+// rows, 228 us for 1208 MB (5.3 TB/s): zeros beside the sort 107, sums 93, long
+// runs 12, the rest marks and launches. Few tokens are bound by their launches: 1024 of 768 bf16
+// into 2048 rows 18.5 us a call.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -38,9 +44,10 @@ bool grouped(const void* p, int dt, int64_t dim, int64_t ld, int n) {
 }
 
 // ---------------------------------------------------------------- lookup
-// One warp per token; a lane takes groups of VEC columns 32 groups apart.
-// Bound by memory: a row read (from L2 when it is met again) and one
-// written per token.
+// One warp per token; a lane takes groups of VEC columns 32 groups apart,
+// kLookupUnroll of them in flight. Bound by memory: a row read (from L2 when
+// it is met again) and one written per token. 131072 tokens of 768 fp32: 88 us,
+// 4.6 TB/s written alone; 24 tokens: 10.4 us a call, the launch.
 constexpr int kLookupWarps = 8;
 constexpr int kLookupUnroll = 4;
 
@@ -219,6 +226,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const int32_t* 
 }
 
 // ------------------------------------------------------ the rows met
+using Mark = uint32_t;
+
 // Number of rows whose first sorted token lies in each tile.
 __global__ void __launch_bounds__(kSortThreads) heads_count_kernel(const uint32_t* __restrict__ keys, int64_t n,
                                                                   int64_t vocab, uint32_t* __restrict__ counts) {
@@ -258,16 +267,15 @@ __global__ void __launch_bounds__(kSortThreads) heads_place_kernel(const uint32_
   }
 }
 
-// Marks every row that a token met, in a byte of its own. Stores to one
-// 32-byte sector queue in L2 (131072 tokens, a quarter of them in the first
-// 32 rows: 19 us), so few blocks take many tokens each, and an id's tokens
-// first meet in a table in the block's shared memory, where all but one
-// usually stay.
+// Marks every row that a token met. Stores to one 32-byte sector queue in L2,
+// so that a row's mark is a word (131072 tokens, a quarter of them in the first
+// 32 rows: 19 us with a byte a row), and an id's tokens first meet in a table
+// in the block's shared memory, where all but one usually stay.
 constexpr int kMarkThreads = 1024;
 constexpr int kMarkBlocks = 32;
 constexpr int kMarkTable = 8192;
 __global__ void __launch_bounds__(kMarkThreads) met_kernel(const int32_t* __restrict__ ids, int64_t n, int64_t vocab,
-                                                          int padding, uint8_t* met) {
+                                                          int padding, Mark* met) {
   __shared__ int table[kMarkTable];
   for (int i = threadIdx.x; i < kMarkTable; i += kMarkThreads) table[i] = -1;
   __syncthreads();
@@ -295,7 +303,9 @@ __global__ void rest_ids_kernel(int32_t* row_ids, int64_t n, const int32_t* coun
 // 19 bits: distributed shared memory moved 5 to 7 bytes a cycle and SM, 14200
 // cycles a pass for the tokens and 9600 for the totals; lanes of one digit
 // found by match_any took 2300 cycles a round (a step for every distinct
-// digit), by a vote a bit 950.
+// digit), by a vote a bit 850. A pass is now 24000 cycles of 131072 tokens
+// (votes 7000, L2 reads at 12 bytes a cycle and SM, which is what the cluster's
+// one GPC gets, 11000), 11000 of 8192; all of it 32 and 11 us.
 constexpr int kGroupThreads = 1024;
 constexpr int kGroupWarps = kGroupThreads / 32;
 constexpr int kRadix = 1 << kMaxDigit;
@@ -314,7 +324,7 @@ struct GroupArgs {
   uint32_t* totals;  // [kMaxBlocks, kWords], two 16-bit totals each, and kMaxBlocks more
   uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
   uint32_t* pos[2];
-  uint8_t* met;      // a byte for every row, 1 where a token met it; null: not asked for
+  Mark* met;      // a mark for every row, 1 where a token met it; null: not asked for
   uint32_t* place;   // with row_ids and count: the rows met; null: not asked for
   int32_t* row_ids;
   int32_t* count;
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   let_next_start();
   if (block == 0 && tid == 0) *a.long_runs = 0;
   if (a.met)  // the barriers of the passes come before the first mark
-    for (int64_t i = block * kGroupThreads + tid; i < (a.vocab + 15) / 16; i += blocks * kGroupThreads)
+    for (int64_t i = block * kGroupThreads + tid; i < (a.vocab + 3) / 4; i += blocks * kGroupThreads)
       __stcg(reinterpret_cast<uint4*>(a.met) + i, make_uint4(0, 0, 0, 0));
   uint2 mine[ITEMS];  // (key, position) of consecutive tokens of a warp, 32 a round
 #pragma unroll
@@ -547,7 +557,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) counted_group_kernel(GroupAr
   let_next_start();
   if (thread == 0) *a.long_runs = 0;
   if (a.met)  // the cluster's barrier comes before the first mark
-    for (int64_t i = thread; i < (a.vocab + 15) / 16; i += threads)
+    for (int64_t i = thread; i < (a.vocab + 3) / 4; i += threads)
       __stcg(reinterpret_cast<uint4*>(a.met) + i, make_uint4(0, 0, 0, 0));
   const int padded = (a.n + 127) / 128 * 128;
   for (int i = tid; i < padded; i += kGroupThreads)
@@ -708,7 +718,7 @@ struct SumArgs {
   // blocks that zero the rows without tokens, spread among those that sum
   int64_t rows;
   const int32_t* count;  // rows met, of the compact gradient; null: the dense one
-  const uint8_t* met;    // a byte for every row of the dense one, 1: has tokens; null: no tokens
+  const Mark* met;    // a mark for every row of the dense one, 1: has tokens; null: no tokens
   int sum_blocks, zero_blocks;
 };
 
@@ -973,7 +983,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
   const bool marks = !compact && !accumulate && n > 0;
-  const size_t met_bytes = marks ? round256(size_t(vocab)) : 0;
+  const size_t met_bytes = marks ? round256(size_t(vocab) * sizeof(Mark)) : 0;
   const size_t list = round256(size_t(n) * 4), part = round256(size_t(chunks) * dim * 4);
   const bool grouped_here = n <= kMaxGroup;
   const size_t hist = grouped_here ? round256((kMaxBlocks * kWords + kMaxBlocks) * 4)
@@ -991,7 +1001,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   uint32_t* place = static_cast<uint32_t*>(take(list));
   uint32_t* long_runs = static_cast<uint32_t*>(take(list));  // at most one in kMinChunk + 1 tokens begins one
   uint32_t* counts = static_cast<uint32_t*>(take(hist));
-  uint8_t* met = marks ? static_cast<uint8_t*>(take(met_bytes)) : nullptr;
+  Mark* met = marks ? static_cast<Mark*>(take(met_bytes)) : nullptr;
   SumArgs a{};
   a.met = met;
   a.long_runs = long_runs;

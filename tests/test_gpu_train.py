@@ -859,3 +859,39 @@ def test_operators_in_a_graph(cuda):
         got = [o.clone() for o in outs]
         for a, b in zip(got, all_of_them()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n", [7, 1000, 2048, 2049, 5000, 20000])
+@pytest.mark.parametrize("vocab", [1 << 10, (1 << 20) + 3, 2 ** 31 - 2])
+def test_grad_rows_of_wide_keys(cuda, n, vocab):
+    """One to four passes of the sorts that few tokens take."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n)
+    dy = _randn((n, 3), g, cuda)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int64)
+    ids[::3], ids[1::5], ids[2::5] = vocab - 1, 0, -1
+    r = train.EmbeddingGradRows(dy, ids.int(), vocab)
+    keep = ids >= 0
+    met, at = torch.unique(ids[keep], return_inverse=True)
+    d = dy.double()[keep]
+    want = torch.zeros(len(met), 3, dtype=torch.float64, device=cuda).index_add_(0, at, d)
+    size = torch.zeros_like(want).index_add_(0, at, d.abs())
+    assert int(r.Count) == len(met) and torch.equal(r.Ids[:len(met)].long(), met)
+    assert bool((r.Ids[len(met):] == -1).all()) and not r.Rows[len(met):].any()
+    _near(r.Rows[:len(met)], want, (torch.bincount(at).double()[:, None] + 1) * u * size)
+
+
+def test_lookup_of_an_empty_table(cuda):
+    import torch
+
+    from ai_b200 import _lib, train
+
+    y = train.Embedding(torch.empty(0, 5, device=cuda), torch.tensor([-1, -1], dtype=torch.int32, device=cuda))
+    assert y.shape == (2, 5) and not y.any()
+    train.Check(cuda)
+    train.Embedding(torch.empty(0, 5, device=cuda), torch.tensor([0], dtype=torch.int32, device=cuda))
+    with pytest.raises(_lib.FGError):
+        train.Check(cuda)
