@@ -15,8 +15,8 @@
 //
 // Bound by memory for many tokens: 131072 of 768 fp32 into a table of 262144
 // rows, 228 us for 1208 MB (5.3 TB/s): zeros beside the sort 107, sums 93, long
-// runs 12, the rest marks and launches. Few tokens are bound by their launches: 1024 of 768 bf16
-// into 2048 rows 18.5 us a call.
+// runs 12, the rest marks and launches. Few tokens are bound by three dependent
+// launches: 1024 of 768 bf16 into 2048 rows 18.5 us a call.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -324,7 +324,7 @@ struct GroupArgs {
   uint32_t* totals;  // [kMaxBlocks, kWords], two 16-bit totals each, and kMaxBlocks more
   uint32_t* key[2];  // passes write them in turn, the last one key[0] and pos[0]
   uint32_t* pos[2];
-  Mark* met;      // a mark for every row, 1 where a token met it; null: not asked for
+  Mark* met;         // a mark for every row, 1 where a token met it; null: not asked for
   uint32_t* place;   // with row_ids and count: the rows met; null: not asked for
   int32_t* row_ids;
   int32_t* count;
@@ -375,7 +375,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = gridDim.x, block = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr uint32_t mask = kRadix - 1;
   let_next_start();
   if (block == 0 && tid == 0) *a.long_runs = 0;
   if (a.met)  // the barriers of the passes come before the first mark
@@ -464,7 +463,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     const uint16_t* offset = reinterpret_cast<const uint16_t*>(sh.offset[warp / kHalfWarps]);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t d = (mine[k].x >> shift) & mask;
+      const uint32_t d = (mine[k].x >> shift) & (kRadix - 1);
       rank[k] += sh.start[d] + offset[d] + count[d];
     }
     __syncthreads();  // the counters are read: their memory takes the tokens
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
     for (int k = 0; k < ITEMS; ++k) {
       const int at = k * kGroupThreads + tid;
       const uint2 it = sh.local[at];
-      const uint32_t to = sh.base[(it.x >> shift) & mask] + at;
+      const uint32_t to = sh.base[(it.x >> shift) & (kRadix - 1)] + at;
       if (to < uint32_t(a.n)) {
         __stcg(key_to + to, it.x);
         __stcg(pos_to + to, it.y);
@@ -686,6 +685,14 @@ __device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, 
 }
 
 // ------------------------------------------------------------------ sums
+constexpr int kMaxChunk = 32;  // tokens: a lane for each
+constexpr int kMinChunk = 4;
+constexpr int kRing = 4;       // rows in flight where tokens are summed
+constexpr int kAhead = 8;      // partial sums in flight where they are joined
+constexpr int kSumWarps = 8;
+// Bytes of a dense gradient from which its zeros are written beside the sort.
+constexpr int64_t kZerosFirst = int64_t(32) << 20;
+
 // A warp sums one chunk of sorted tokens over 32·VEC columns, with kRing
 // rows in flight (4, 6 and 8 of them, with the warps that their registers
 // leave room for, measured alike). A run of one id no longer than a chunk
@@ -694,14 +701,6 @@ __device__ __forceinline__ int64_t first_token(const uint32_t* keys, int64_t n, 
 // goes to tail[chunk], the others to head[chunk], and join_kernel adds them.
 // (Runs of any length cut at the chunks' ends: four times as many to join,
 // 23 us of 131072 frequent tokens' 240.)
-// Bytes of a dense gradient from which its zeros are written beside the sort.
-constexpr int64_t kZerosFirst = int64_t(32) << 20;
-constexpr int kMaxChunk = 32;
-constexpr int kMinChunk = 4;
-constexpr int kRing = 4;
-constexpr int kAhead = 8;  // partial sums in flight where they are joined
-constexpr int kSumWarps = 8;
-
 struct SumArgs {
   const uint32_t* keys;
   const uint32_t* pos;
@@ -718,7 +717,7 @@ struct SumArgs {
   // blocks that zero the rows without tokens, spread among those that sum
   int64_t rows;
   const int32_t* count;  // rows met, of the compact gradient; null: the dense one
-  const Mark* met;    // a mark for every row of the dense one, 1: has tokens; null: no tokens
+  const Mark* met;       // a mark for every row of the dense one, 1: has tokens; null: no tokens
   int sum_blocks, zero_blocks;
 };
 
@@ -976,9 +975,9 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   const int digit = (bits + passes - 1) / passes;
   const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
   const int slices = int(blocks_of(dim, wide ? 128 : 32));
-  // few tokens are cut into shorter chunks, down to kMinChunk, until there is a
-  // warp for every quarter of an SM's: a chunk's rows arrive kRing at a time
-  // (1024 tokens x 768 bf16: 16 us in chunks of 32, 10 us in chunks of 4)
+  // few tokens are cut into shorter chunks, down to kMinChunk, until there are
+  // 16 warps an SM: a chunk's rows arrive kRing at a time (the sums of 333
+  // tokens x 256 fp32: 11 us in chunks of 32, 6.8 us in chunks of 4)
   int chunk = kMaxChunk;
   while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
