@@ -542,27 +542,30 @@ struct LogProbsGradArgs {
   int* err;
 };
 
-// Elementwise: a block takes kGradGroups 16-byte groups a thread of one row,
-// all loaded before the first is used; groups are those of the logits'
-// memory, stored whole where the gradient's lie alike.
-constexpr int kGradThreads = 256;
+// Elementwise: a warp takes kGradGroups 16-byte groups a lane of one row, all
+// loaded before the first is used; groups are those of the logits' memory,
+// stored whole where the gradient's lie alike.
+constexpr int kGradWarps = 8;
 constexpr int kGradGroups = 4;
 
 template <typename T, bool ENTROPY>
-__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(LogProbsGradArgs a, int parts, const T* logits,
-                                                                    T* dlogits) {
+__global__ void __launch_bounds__(kGradWarps * 32) logprobs_grad_kernel(LogProbsGradArgs a, int parts, const T* logits,
+                                                                       T* dlogits) {
   constexpr int V = 16 / int(sizeof(T));
-  const int64_t row = blockIdx.x / parts;
-  const int part = blockIdx.x % parts;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(blockIdx.x) * kGradWarps + (threadIdx.x >> 5);
+  const int64_t row = unit / parts;
+  const int part = int(unit % parts);
+  if (row >= a.rows) return;
   const T* x = logits + row * a.ld;
   T* dx = dlogits + row * a.ldd;
   const int skip = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
-  const int64_t j0 = (int64_t(part) * (kGradThreads * kGradGroups) + threadIdx.x) * V - skip;
+  const int64_t j0 = (int64_t(part) * (32 * kGradGroups) + lane) * V - skip;
   Pack<T, V> in[kGradGroups];
 #pragma unroll
   for (int g = 0; g < kGradGroups; ++g) {
-    const int64_t j = j0 + g * kGradThreads * V;
+    const int64_t j = j0 + g * 32 * V;
     if (j >= 0 && j + V <= a.width) {
       in[g].load_own(x + j);
     } else {
@@ -571,7 +574,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(LogProbsGra
     }
   }
   const int t = a.targets[row];
-  if (t >= a.width && part == 0 && threadIdx.x == 0) atomicCAS(a.err, 0, kDevBadIndex);
+  if (t >= a.width && part == 0 && lane == 0) atomicCAS(a.err, 0, kDevBadIndex);
   const bool none = t < 0 || t >= a.width;
   const float lse = a.lse[row];
   const float g0 = none ? 0.f : a.dlogprob[row];
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(LogProbsGra
   }
 #pragma unroll
   for (int g = 0; g < kGradGroups; ++g) {
-    const int64_t j = j0 + g * kGradThreads * V;
+    const int64_t j = j0 + g * 32 * V;
     if (j >= a.width) break;
     Pack<T, V> out;
 #pragma unroll
@@ -608,25 +611,25 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(LogProbsGra
 
 template <typename T>
 int launch_logprobs_grad(const LogProbsGradArgs& a, const T* logits, T* dlogits, cudaStream_t s) {
-  constexpr int V = 16 / int(sizeof(T)), kPart = kGradThreads * kGradGroups * V;
+  constexpr int V = 16 / int(sizeof(T)), kPart = 32 * kGradGroups * V;
   // a row that begins inside a 16-byte group reaches into one more
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && a.ld % V == 0;
   const int64_t parts = (int64_t(a.width) + (aligned ? 0 : V - 1) + kPart - 1) / kPart;
   // rows that one launch's grid holds; more only past 2^31 blocks
-  const int64_t most = INT32_MAX / parts;
+  const int64_t most = int64_t(INT32_MAX) * kGradWarps / parts;
   for (int64_t r = 0; r < a.rows; r += most) {
     LogProbsGradArgs b = a;
     b.rows = std::min(most, a.rows - r);
     b.targets += r;
     b.lse += r;
     b.dlogprob += r;
-    const unsigned blocks = unsigned(b.rows * parts);
+    const unsigned blocks = unsigned((b.rows * parts + kGradWarps - 1) / kGradWarps);
     if (a.dentropy) {
       b.dentropy += r;
       b.entropy += r;
-      logprobs_grad_kernel<T, true><<<blocks, kGradThreads, 0, s>>>(b, int(parts), logits + r * a.ld, dlogits + r * a.ldd);
+      logprobs_grad_kernel<T, true><<<blocks, kGradWarps * 32, 0, s>>>(b, int(parts), logits + r * a.ld, dlogits + r * a.ldd);
     } else {
-      logprobs_grad_kernel<T, false><<<blocks, kGradThreads, 0, s>>>(b, int(parts), logits + r * a.ld, dlogits + r * a.ldd);
+      logprobs_grad_kernel<T, false><<<blocks, kGradWarps * 32, 0, s>>>(b, int(parts), logits + r * a.ld, dlogits + r * a.ldd);
     }
     FG_CUDA_TRY(cudaGetLastError());
   }

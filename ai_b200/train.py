@@ -225,7 +225,8 @@ def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
                  scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The logits' gradient of ``LogProbs`` from its LogSum (and Entropy) and
     the gradients of its log probabilities and, where ``dentropy`` is given,
-    of its entropies. ``out`` may be the logits themselves."""
+    of its entropies. ``out`` may be the logits themselves; a new tensor has
+    their rows' distance where that is little more than their length."""
     op = "LogProbsGrad"
     code, x, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
     lse = _float32(op, "lse", lse, rows, index)
@@ -238,7 +239,11 @@ def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
         entropy = _float32(op, "entropy", entropy, rows, index)
         entropy_at, dentropy_at = entropy.data_ptr(), dentropy.data_ptr()
     if out is None:
-        out, ldo = x.new_empty((rows, width)), width
+        # rows as far apart as the logits' own, so that both lie alike in memory
+        ldo = ld if ld - width < 64 else width
+        out = x.new_empty((rows, ldo))
+        if ldo != width:
+            out = out[:, :width]
     else:
         if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.get_device() != index or out.shape != x.shape:
             _fail(op, f"out must be {x.dtype} [{rows}, {width}] on cuda:{index}")
