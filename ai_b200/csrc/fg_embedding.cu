@@ -564,12 +564,20 @@ __global__ void __launch_bounds__(kGroupThreads, 1) counted_group_kernel(GroupAr
   __syncthreads();
   for (int i = block * kGroupWarps + warp; i < a.n; i += gridDim.x * kGroupWarps) {
     const uint32_t mine = keys[i];
+    // keys up to its own count among earlier tokens, keys below it among later
+    // ones: k < mine + 1 before token i's 128, k < mine behind them
     int before = 0;
+    auto count = [&](int from, int to, uint32_t limit) {
 #pragma unroll 4
-    for (int j = lane * 4; j < padded; j += 128) {
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
-      before += (k.x < mine + (j < i)) + (k.y < mine + (j + 1 < i)) + (k.z < mine + (j + 2 < i)) + (k.w < mine + (j + 3 < i));
-    }
+      for (int j = from + lane * 4; j < to; j += 128) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+        before += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+      }
+    };
+    const int own = i / 128 * 128;
+    count(0, own, mine + 1);
+    count(own + 128, padded, mine);
+    for (int j = own + lane; j < own + 128; j += 32) before += keys[j] < mine + (j < i);
     before = __reduce_add_sync(kFull, before);
     if (lane == 0) {
       __stcg(a.key[0] + before, mine);
