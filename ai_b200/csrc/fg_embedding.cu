@@ -5,18 +5,19 @@
 //   lookup:   y[t] = scale · W[id_t]
 //   gradient: G[v] = scale · Σ_{t : id_t = v} dy[t]
 //
-// The gradient sorts the tokens by id, stably, so a row's tokens stay in
-// their order (by counting up to 2048 tokens, within one cluster up to 262144,
-// through memory beyond); cuts the sorted tokens into chunks of equal length
-// however often a token occurs; sums the runs of one id in registers; and
-// joins the runs that are longer than a chunk in a second kernel. Sums are in
-// 32 bits in an order that depends on the ids alone, so a repeated call gives
-// the same bits; a sum is rounded once, when its row is written.
+// Up to 2048 tokens the gradient is one launch whose blocks group the tokens in
+// a hash table each. More are sorted by id, stably, so a row's tokens stay in
+// their order (within one cluster up to 262144, through memory beyond), and
+// cut into chunks of equal length however often a token occurs; the runs of
+// one id are summed in registers, and those longer than a chunk joined in a
+// second kernel. Sums are in 32 bits in an order that depends on the ids
+// alone, so a repeated call gives the same bits; a sum is rounded once, when
+// its row is written.
 //
 // Bound by memory for many tokens: 131072 of 768 fp32 into a table of 262144
 // rows, 228 us for 1208 MB (5.3 TB/s): zeros beside the sort 107, sums 93, long
-// runs 12, the rest marks and launches. Few tokens are bound by three dependent
-// launches: 1024 of 768 bf16 into 2048 rows 18.5 us a call.
+// runs 12, the rest marks and launches. 1024 of 768 bf16 into 2048 rows: 15 us
+// a call, the latency of one kernel.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -539,101 +540,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   if (block == 0 && tid == 0) *a.count = int32_t(total);
 }
 
-// ---------------------------------------------------- few tokens: counting
-// A token's place in the sorted order is the number of tokens before it there,
-// those with a smaller key and those of its own key that come earlier. With
-// n <= kMaxCounted every warp counts a token's over all keys in shared memory,
-// n^2 comparisons spread over a cluster's blocks and no pass that waits for
-// another: 333 tokens 6.5 us, by digits in one block 13.3 (profiled launches).
-constexpr int kMaxCounted = 2048;
-
-__global__ void __launch_bounds__(kGroupThreads, 1) counted_group_kernel(GroupArgs a) {
-  __shared__ __align__(16) uint32_t keys[kMaxCounted];
-  __shared__ uint32_t warp_sum[kGroupWarps];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int block = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int thread = block * kGroupThreads + tid, threads = gridDim.x * kGroupThreads;
-  let_next_start();
-  if (thread == 0) *a.long_runs = 0;
-  if (a.met)  // the cluster's barrier comes before the first mark
-    for (int64_t i = thread; i < (a.vocab + 3) / 4; i += threads)
-      __stcg(reinterpret_cast<uint4*>(a.met) + i, make_uint4(0, 0, 0, 0));
-  const int padded = (a.n + 127) / 128 * 128;
-  for (int i = tid; i < padded; i += kGroupThreads)
-    keys[i] = i < a.n ? token_key(a.ids[i], a.vocab, a.padding, a.err) : 0xffffffffu;
-  __syncthreads();
-  for (int i = block * kGroupWarps + warp; i < a.n; i += gridDim.x * kGroupWarps) {
-    const uint32_t mine = keys[i];
-    // keys up to its own count among earlier tokens, keys below it among later
-    // ones: k < mine + 1 before token i's 128, k < mine behind them
-    int before = 0;
-    auto count = [&](int from, int to, uint32_t limit) {
-#pragma unroll 4
-      for (int j = from + lane * 4; j < to; j += 128) {
-        const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
-        before += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
-      }
-    };
-    const int own = i / 128 * 128;
-    count(0, own, mine + 1);
-    count(own + 128, padded, mine);
-    for (int j = own + lane; j < own + 128; j += 32) before += keys[j] < mine + (j < i);
-    before = __reduce_add_sync(kFull, before);
-    if (lane == 0) {
-      __stcg(a.key[0] + before, mine);
-      __stcg(a.pos[0] + before, uint32_t(i));
-    }
-  }
-  cluster.sync();
-  // where the rows begin
-  auto key_at = [&](int i) { return i >= 0 && i < a.n ? __ldcg(a.key[0] + i) : 0xffffffffu; };
-  if (a.met && thread < a.n) {
-    const uint32_t key = key_at(thread);
-    if (key < a.vocab && key != key_at(thread - 1)) a.met[key] = 1;
-  }
-  if (!a.place || block > 0) return;
-  constexpr int kEach = kMaxCounted / kGroupThreads;
-  uint32_t key[kEach], heads = 0;
-  bool head[kEach];
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = tid * kEach + k;
-    key[k] = key_at(i);
-    head[k] = key[k] < a.vocab && key[k] != key_at(i - 1);
-    heads += head[k];
-  }
-  uint32_t total;
-  uint32_t upto = block_scan(heads, warp_sum, &total);
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = tid * kEach + k;
-    upto += head[k];
-    if (i >= a.n) continue;
-    if (key[k] < a.vocab) a.place[i] = upto - 1;
-    if (head[k]) a.row_ids[upto - 1] = int32_t(key[k]);
-    if (uint32_t(i) >= total) a.row_ids[i] = -1;
-  }
-  if (tid == 0) *a.count = int32_t(total);
-}
-
-// A kernel over one cluster of `blocks` blocks.
-template <typename Kernel>
-int launch_cluster(Kernel kernel, const GroupArgs& a, int blocks, size_t shared, cudaStream_t s) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(blocks);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(blocks));
-  cfg.blockDim = dim3(kGroupThreads);
-  cfg.dynamicSmemBytes = shared;
-  cfg.stream = s;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
-  return FG_OK;
-}
-
 template <int ITEMS>
 int launch_group(const GroupArgs& a, int blocks, cudaStream_t s) {
   auto kernel = group_kernel<ITEMS>;
@@ -643,24 +549,25 @@ int launch_group(const GroupArgs& a, int blocks, cudaStream_t s) {
     FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     ready.done();
   }
-  return launch_cluster(kernel, a, blocks, sizeof(GroupShared<ITEMS>), s);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(blocks);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(kGroupThreads);
+  cfg.dynamicSmemBytes = sizeof(GroupShared<ITEMS>);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  return FG_OK;
 }
 
 // Most tokens that a cluster sorts.
 constexpr int64_t kMaxGroup = int64_t(kMaxBlocks) * kGroupThreads * kMaxGroupItems;
 
 int group_tokens(const GroupArgs& a, cudaStream_t s) {
-  if (a.n <= kMaxCounted) {
-    static OncePerDevice ready;
-    if (ready.first()) {
-      FG_CUDA_TRY(cudaFuncSetAttribute(counted_group_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      ready.done();
-    }
-    // a token for every warp, as far as the cluster goes
-    int blocks = 1;
-    while (blocks < kMaxBlocks && blocks * kGroupWarps < a.n) blocks *= 2;
-    return launch_cluster(counted_group_kernel, a, blocks, 0, s);
-  }
   // as many blocks as the tokens fill, then more tokens a thread
   int blocks = 1, items = 1;
   while (blocks < kMaxBlocks && blocks * kGroupThreads < a.n) blocks *= 2;
@@ -983,10 +890,11 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
 // each, looked up in the table, or the token's own place in the compact one
 // where that lies past the last row. No scratch, and one launch instead of
 // three that depend on one another: 1024 tokens x 768 bf16 into 2048 rows
-// took 18.5 us in order of ids, X here.
+// took 18.5 us in order of ids, 15 here; 333 x 256 fp32, rows met, 20 and 14.
 constexpr int kFewTokens = 2048;
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kFewBlocks = 4;  // an SM's
 constexpr int kFewRing = 8;
 constexpr int kWholeRun = 32;  // tokens of a run that one warp sums
 constexpr uint32_t kNoKey = 0xffffffffu;
@@ -1054,108 +962,114 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(FewArgs a, const TY* _
   }
   __syncthreads();
 
-  const int64_t unit = int64_t(blockIdx.x) * kFewWarps + warp;
-  const bool token = unit < a.token_units;
-  const int64_t at = token ? unit : unit - a.token_units;
-  const int col = (int(at % a.slices) * 32 + lane) * VEC;
-  const bool in = col < a.dim && unit < a.units;
-  const int t = token ? int(at / a.slices) : 0;
-  Pack<TG, VEC> zero;
+  for (int64_t base = int64_t(blockIdx.x) * kFewWarps; base < a.units; base += int64_t(gridDim.x) * kFewWarps) {
+    const int64_t unit = base + warp;
+    const bool token = unit < a.token_units;
+    // A frequent id's first token comes early: a block's warps take tokens far
+    // apart, and the columns of a token meet in different blocks.
+    const int64_t at = token ? unit : unit - a.token_units, across = token ? a.words * 32 : (a.rows + 31) / 32;
+    const int slice = int(at / across), place_in = int(at % across);
+    const int col = (slice * 32 + lane) * VEC;
+    const bool in = col < a.dim && unit < a.units;
+    const int t = token ? place_in % kFewWarps * (a.words * 32 / kFewWarps) + place_in / kFewWarps : 0;
+    Pack<TG, VEC> zero;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) zero.set(i, 0.f);
-  if (!token && unit < a.units) {  // 32 rows of the dense gradient
-    const int64_t r0 = at / a.slices * 32;
-    const bool met = r0 + lane < a.rows && find(uint32_t(r0 + lane)) < uint32_t(a.slots);
-    unsigned keep = __ballot_sync(kFull, met);
-    if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
-    TG* g = grad + r0 * a.ldg + col;
-    if (in)
+    for (int i = 0; i < VEC; ++i) zero.set(i, 0.f);
+    if (!token && unit < a.units) {  // 32 rows of the dense gradient
+      const int64_t r0 = int64_t(place_in) * 32;
+      const bool met = r0 + lane < a.rows && find(uint32_t(r0 + lane)) < uint32_t(a.slots);
+      unsigned keep = __ballot_sync(kFull, met);
+      if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
+      TG* g = grad + r0 * a.ldg + col;
+      if (in)
 #pragma unroll 8
-      for (int r = 0; r < 32; ++r)
-        if (!(keep >> r & 1)) zero.store(g + r * a.ldg);
-  }
-  // first tokens of a smaller key; of any key
-  auto firsts_below = [&](uint32_t key) {
-    int c = 0;
-    for (int w = 0; w < a.words; ++w) c += (firsts[w] >> lane & 1) && keys[w * 32 + lane] < key;
-    return __reduce_add_sync(kFull, c);
-  };
-  const bool first = token && (firsts[t / 32] >> t % 32 & 1);
-  const uint32_t key = first ? keys[t] : 0;
-  const int run = first ? int(slot_count[find(key)]) : 0;
-  int64_t row = key;
-  if (a.count && token) {
-    if (first) row = firsts_below(key);
-    const int met = firsts_below(kNoKey);
-    const bool names = at % a.slices == 0 && lane == 0;
-    if (first && names) a.row_ids[row] = int32_t(key);
-    if (t >= met) {
-      if (in) zero.store(grad + int64_t(t) * a.ldg + col);
-      if (names) a.row_ids[t] = -1;
+        for (int r = 0; r < 32; ++r)
+          if (!(keep >> r & 1)) zero.store_past(g + r * a.ldg);
     }
-    if (t == 0 && names) *a.count = met;
-  }
-  // sums the tokens of a key within some words of tokens, in their order
-  const TY* y = dy + col;
-  auto sum = [&](float (&acc)[VEC], uint32_t of, int word, int end, bool with) {
-    int found = 0;
-    for (; word < end; ++word) {
-      const bool mine = keys[word * 32 + lane] == of;
-      const unsigned who = __ballot_sync(kFull, mine);
-      if (mine) list[warp][found + __popc(who & ((1u << lane) - 1))] = uint16_t(word * 32 + lane);
-      found += __popc(who);
+    if (base >= a.token_units) continue;  // zeros alone: no barrier
+    // first tokens of a smaller key; of any key
+    auto firsts_below = [&](uint32_t key) {
+      int c = 0;
+      for (int w = 0; w < a.words; ++w) c += (firsts[w] >> lane & 1) && keys[w * 32 + lane] < key;
+      return __reduce_add_sync(kFull, c);
+    };
+    const bool first = token && (firsts[t / 32] >> t % 32 & 1);
+    const uint32_t key = first ? keys[t] : 0;
+    const int run = first ? int(slot_count[find(key)]) : 0;
+    int64_t row = key;
+    if (a.count && token && t < a.n) {
+      if (first) row = firsts_below(key);
+      const int met = firsts_below(kNoKey);
+      const bool names = slice == 0 && lane == 0;
+      if (first && names) a.row_ids[row] = int32_t(key);
+      if (t >= met) {
+        if (in) zero.store(grad + int64_t(t) * a.ldg + col);
+        if (names) a.row_ids[t] = -1;
+      }
+      if (t == 0 && names) *a.count = met;
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    for (int i0 = 0; i0 < found; i0 += kFewRing) {
-      Pack<TY, VEC> v[kFewRing];
-#pragma unroll
-      for (int u = 0; u < kFewRing; ++u)
-        if (i0 + u < found && with) v[u].load(y + int64_t(list[warp][i0 + u]) * a.ldy);
-#pragma unroll
-      for (int u = 0; u < kFewRing; ++u)
-        if (i0 + u < found)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
-    }
-    __syncwarp();  // the list is read until here
-  };
-  float acc[VEC];
-  if (first && run <= kWholeRun) {
-    if (run == 1) {
-      Pack<TY, VEC> v;
-      if (in) v.load(y + int64_t(t) * a.ldy);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = v.get(i);
-    } else {
-      sum(acc, key, t / 32, a.words, in);
-    }
-    if (in) write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
-  }
-  if (lane == 0) shared_unit[warp] = first && run > kWholeRun ? t : -1;
-  __syncthreads();
-  for (int w = 0; w < kFewWarps; ++w) {
-    const int of = shared_unit[w];
-    if (of < 0) continue;
-    const int share = (a.words + kFewWarps - 1) / kFewWarps, word = min(a.words, warp * share);
-    // the columns are the unit's, not this warp's own
-    const int64_t theirs = int64_t(blockIdx.x) * kFewWarps + w;
-    const int c = (int(theirs % a.slices) * 32 + lane) * VEC;
-    y = dy + c;
-    sum(acc, keys[of], word, min(a.words, word + share), c < a.dim);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) part[warp][lane * VEC + i] = acc[i];
-    __syncthreads();
-    if (warp == w && in) {
+    // sums the tokens of a key within some words of tokens, in their order
+    const TY* y = dy + col;
+    auto sum = [&](float (&acc)[VEC], uint32_t of, int word, int end, bool with) {
+      int found = 0;
+      for (; word < end; ++word) {
+        const bool mine = keys[word * 32 + lane] == of;
+        const unsigned who = __ballot_sync(kFull, mine);
+        if (mine) list[warp][found + __popc(who & ((1u << lane) - 1))] = uint16_t(word * 32 + lane);
+        found += __popc(who);
+      }
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-      for (int p = 0; p < kFewWarps; ++p)
+      for (int i0 = 0; i0 < found; i0 += kFewRing) {
+        Pack<TY, VEC> v[kFewRing];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += part[p][lane * VEC + i];
-      write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
+        for (int u = 0; u < kFewRing; ++u)
+          if (i0 + u < found && with) v[u].load(y + int64_t(list[warp][i0 + u]) * a.ldy);
+#pragma unroll
+        for (int u = 0; u < kFewRing; ++u)
+          if (i0 + u < found)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] += v[u].get(i);
+      }
+      __syncwarp();  // the list is read until here
+    };
+    float acc[VEC];
+    if (first && run <= kWholeRun) {
+      if (run == 1) {
+        Pack<TY, VEC> v;
+        if (in) v.load(y + int64_t(t) * a.ldy);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = v.get(i);
+      } else {
+        sum(acc, key, t / 32, a.words, in);
+      }
+      if (in) write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
     }
+    if (lane == 0) shared_unit[warp] = first && run > kWholeRun ? t : -1;
     __syncthreads();
+    for (int w = 0; w < kFewWarps; ++w) {
+      const int of = shared_unit[w];
+      if (of < 0) continue;
+      const int share = (a.words + kFewWarps - 1) / kFewWarps, word = min(a.words, warp * share);
+      // the columns are the unit's, not this warp's own
+      const int c = (int((base + w) / (a.words * 32)) * 32 + lane) * VEC;
+      y = dy + c;
+      sum(acc, keys[of], word, min(a.words, word + share), c < a.dim);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) part[warp][lane * VEC + i] = acc[i];
+      __syncthreads();
+      if (warp == w && in) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+        for (int p = 0; p < kFewWarps; ++p)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[i] += part[p][lane * VEC + i];
+        write_row<TG, VEC>(grad + row * a.ldg + col, acc, a.scale, a.accumulate);
+      }
+      __syncthreads();
+    }
+    __syncthreads();  // shared_unit is read until here
   }
 }
 
@@ -1199,12 +1113,13 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     f.ldg = ldg;
     f.scale = scale;
     f.accumulate = accumulate;
-    f.token_units = n * slices;
+    f.token_units = int64_t(f.words) * 32 * slices;
     f.units = f.token_units + (compact || accumulate ? 0 : blocks_of(vocab, 32) * slices);
     f.row_ids = row_ids;
     f.count = count;
     f.err = err;
-    const unsigned blocks = unsigned(blocks_of(f.units, kFewWarps));
+    // no more blocks than run at once: each makes the table again
+    const unsigned blocks = unsigned(std::min<int64_t>(blocks_of(f.units, kFewWarps), int64_t(sm_count()) * kFewBlocks));
     const size_t shared = few_shared(f.words, f.slots);
     return by_dtype(grad_dtype, [&](auto tg) {
       return by_dtype(dy_dtype, [&](auto ty) {
@@ -1232,8 +1147,8 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   const int passes = (bits + kMaxDigit - 1) / kMaxDigit;
   const int digit = (bits + passes - 1) / passes;
   // few tokens are cut into shorter chunks, down to kMinChunk, until there are
-  // 16 warps an SM: a chunk's rows arrive kRing at a time (the sums of 333
-  // tokens x 256 fp32: 11 us in chunks of 32, 6.8 us in chunks of 4)
+  // 16 warps an SM: a chunk's rows arrive kRing at a time (measured on 333 tokens
+  // x 256 fp32 in this form: sums 11 us in chunks of 32, 6.8 in chunks of 4)
   int chunk = kMaxChunk;
   while (chunk > kMinChunk && blocks_of(n, chunk) * slices < int64_t(sm_count()) * 16) chunk /= 2;
   const int64_t tiles = blocks_of(n, kSortTile), chunks = blocks_of(n, chunk);
@@ -1264,7 +1179,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.tail = static_cast<float*>(take(part));
   // A large dense gradient's zeros are written while a cluster sorts (16 of the
   // SMs); the rows met are then marked beforehand.
-  const bool zeros_first = met && grouped_here && n > kMaxCounted && vocab * dim * dtype_size(grad_dtype) >= kZerosFirst;
+  const bool zeros_first = met && grouped_here && vocab * dim * dtype_size(grad_dtype) >= kZerosFirst;
   if (zeros_first || (met && !grouped_here)) {
     FG_CUDA_TRY(cudaMemsetAsync(met, 0, met_bytes, s));
     met_kernel<<<kMarkBlocks, kMarkThreads, 0, s>>>(ids, n, vocab, padding, met);
