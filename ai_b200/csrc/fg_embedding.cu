@@ -16,7 +16,7 @@
 //
 // Bound by memory for many tokens: 131072 of 768 fp32 into a table of 262144
 // rows, 228 us for 1208 MB (5.3 TB/s): zeros beside the sort 107, sums 93, long
-// runs 12, the rest marks and launches. 1024 of 768 bf16 into 2048 rows: 15 us
+// runs 12, the rest marks and launches. 1024 of 768 bf16 into 2048 rows: 14.4 us
 // a call, the latency of one kernel.
 #include <cooperative_groups.h>
 
@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
 // each, looked up in the table, or the token's own place in the compact one
 // where that lies past the last row. No scratch, and one launch instead of
 // three that depend on one another: 1024 tokens x 768 bf16 into 2048 rows
-// took 18.5 us in order of ids, 15 here; 333 x 256 fp32, rows met, 20 and 14.
+// took 18.5 us in order of ids, 14.4 here; 333 x 256 fp32, rows met, 20 and 14.5.
 constexpr int kFewTokens = 2048;
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
@@ -986,7 +986,6 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(FewArgs a, const TY* _
         for (int r = 0; r < 32; ++r)
           if (!(keep >> r & 1)) zero.store_past(g + r * a.ldg);
     }
-    if (base >= a.token_units) continue;  // zeros alone: no barrier
     // first tokens of a smaller key; of any key
     auto firsts_below = [&](uint32_t key) {
       int c = 0;
