@@ -651,26 +651,60 @@ __device__ __forceinline__ void write_row(TG* g, const float (&acc)[VEC], float 
   r.store(g);
 }
 
+// Zeros in n consecutive values from anywhere, by a warp: whole 16 bytes but
+// for the ends.
+template <typename T>
+__device__ __forceinline__ void zero_values(T* p, int64_t n, int lane) {
+  constexpr int V = 16 / int(sizeof(T));
+  const int64_t before = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T);
+  const int64_t head = n < before ? n : before, groups = (n - head) / V, tail = head + groups * V;
+  for (int64_t g = lane; g < groups; g += 32) __stcs(reinterpret_cast<uint4*>(p + head) + g, make_uint4(0, 0, 0, 0));
+  if (lane < head) p[lane] = narrow<T>(0.f);
+  if (tail + lane < n) p[tail + lane] = narrow<T>(0.f);
+}
+
+// Zeros in those of 32 rows whose bit of `keep` is 0, by a warp: the columns
+// of its slice (col) where values are stored in fours; else whole rows, those
+// that follow one another in one go (20000 tokens into 262144 x 129 bf16
+// took 64 us one value a lane, 45 this way; 5000 into 60000 x 301 fp32 43 and
+// 37).
+template <typename TG, int VEC>
+__device__ __forceinline__ void zero_kept(TG* rows, unsigned keep, int col, int dim, int64_t ldg, int lane) {
+  if (VEC == 1) {
+    for (int r = 0; r < 32;) {
+      const unsigned left = ~keep >> r;
+      if (left == 0) return;
+      r += __ffs(left) - 1;
+      const int more = __ffs(~(~keep >> r)) - 1, run = ldg != dim ? 1 : more < 0 ? 32 - r : more;
+      zero_values(rows + r * ldg, int64_t(run) * dim, lane);
+      r += run;
+    }
+    return;
+  }
+  if (col >= dim) return;
+  Pack<TG, VEC> z;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
+  TG* g = rows + col;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r)
+    if (!(keep >> r & 1)) z.store_past(g + r * ldg);
+}
+
 // Zeros in the rows of the dense gradient that no token met (there may be
 // no tokens at all), or past the last row of the compact one: a warp takes
-// 32·VEC columns of 32 rows.
+// 32·VEC columns of 32 rows, or the rows whole.
 template <typename TG, int VEC>
 __device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t unit, TG* grad, int lane) {
-  const int64_t r0 = unit / a.slices * 32;
-  const int col = (int(unit % a.slices) * 32 + lane) * VEC;
+  const int slices = VEC == 1 ? 1 : a.slices;
+  const int64_t r0 = unit / slices * 32;
+  const int col = (int(unit % slices) * 32 + lane) * VEC;
   if (r0 >= a.rows) return;
   const int64_t count = a.count ? int64_t(*a.count) - r0 : 0;
   unsigned keep = count >= 32 ? kFull : count > 0 ? (1u << count) - 1 : 0;
   if (!a.count && a.met) keep = __ballot_sync(kFull, r0 + lane < a.rows && a.met[r0 + lane]);
   if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
-  if (col >= a.dim) return;
-  Pack<TG, VEC> z;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) z.set(i, 0.f);
-  TG* g = grad + r0 * a.ldg + col;
-#pragma unroll 8
-  for (int r = 0; r < 32; ++r)
-    if (!(keep >> r & 1)) z.store_past(g + r * a.ldg);
+  zero_kept<TG, VEC>(grad + r0 * a.ldg, keep, col, a.dim, a.ldg, lane);
 }
 
 // The zeros alone, while the tokens are sorted: needs the marks of the rows
@@ -891,7 +925,15 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
 // where that lies past the last row. No scratch, and one launch instead of
 // three that depend on one another: 1024 tokens x 768 bf16 into 2048 rows
 // took 18.5 us in order of ids, 14.4 here; 333 x 256 fp32, rows met, 20 and 14.5.
+// But a first token looks through all ids in every slice of its columns, so
+// that the work grows with tokens^2 x slices: up to kFewWork of that, beyond it
+// the order of ids is cheaper. A call, here and sorted: 1024 x 1024 bf16 14.6
+// and 20.8 us, rows met 18.7 and 23.2 (8M); 1500 x 512 20.8 and 21.2, 25.1 and
+// 24.0 (9M); 1024 x 301 fp32 18.0 and 20.9, 21.0 and 24.8 (10M); 1500 x 768
+// bf16 23.0 and 21.3, 32.6 and 23.3 (13M); 2048 x 1023 fp32 105 and 25, 168
+// and 35 (128M).
 constexpr int kFewTokens = 2048;
+constexpr int64_t kFewWork = 10 << 20;
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewBlocks = 4;  // an SM's
@@ -980,11 +1022,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(FewArgs a, const TY* _
       const bool met = r0 + lane < a.rows && find(uint32_t(r0 + lane)) < uint32_t(a.slots);
       unsigned keep = __ballot_sync(kFull, met);
       if (a.rows - r0 < 32) keep |= kFull << (a.rows - r0);
-      TG* g = grad + r0 * a.ldg + col;
-      if (in)
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r)
-          if (!(keep >> r & 1)) zero.store_past(g + r * a.ldg);
+      zero_kept<TG, VEC>(grad + r0 * a.ldg, keep, col, a.dim, a.ldg, lane);
     }
     // first tokens of a smaller key; of any key
     auto firsts_below = [&](uint32_t key) {
@@ -1096,7 +1134,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   }
   const bool wide = grouped(dy, dy_dtype, dim, ldy, 4) && grouped(grad, grad_dtype, dim, ldg, 4);
   const int slices = int(blocks_of(dim, wide ? 128 : 32));
-  if (n > 0 && n <= kFewTokens) {
+  if (n > 0 && n <= kFewTokens && n * n * slices <= kFewWork) {
     FewArgs f{};
     f.ids = ids;
     f.n = int(n);
@@ -1113,7 +1151,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     f.scale = scale;
     f.accumulate = accumulate;
     f.token_units = int64_t(f.words) * 32 * slices;
-    f.units = f.token_units + (compact || accumulate ? 0 : blocks_of(vocab, 32) * slices);
+    f.units = f.token_units + (compact || accumulate ? 0 : blocks_of(vocab, 32) * (wide ? slices : 1));
     f.row_ids = row_ids;
     f.count = count;
     f.err = err;
@@ -1220,7 +1258,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   a.rows = compact ? n : vocab;
   a.count = count;
   const int64_t sum_blocks = blocks_of(chunks * blocks_of(slices, wide ? 1 : kNarrowParts), kSumWarps);
-  const int64_t all_zero_blocks = accumulate ? 0 : blocks_of(blocks_of(a.rows, 32) * slices, kSumWarps);
+  const int64_t all_zero_blocks = accumulate ? 0 : blocks_of(blocks_of(a.rows, 32) * (wide ? slices : 1), kSumWarps);
   const int64_t zero_blocks = zeros_first ? 0 : all_zero_blocks;
   if (sum_blocks + zero_blocks > INT32_MAX) return set_error(FG_EINVAL, "embedding gradient: too many tokens times columns");
   if (sum_blocks + zero_blocks == 0) return FG_OK;

@@ -895,3 +895,46 @@ def test_lookup_of_an_empty_table(cuda):
     train.Embedding(torch.empty(0, 5, device=cuda), torch.tensor([0], dtype=torch.int32, device=cuda))
     with pytest.raises(_lib.FGError):
         train.Check(cuda)
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(1024, 700, 301), (1025, 700, 301), (2048, 900, 1023), (1500, 3, 517),
+                                         (2048, 50, 2048), (2047, 5000, 385), (1, 70, 33000), (300, 40, 4097)])
+def test_grad_of_few_tokens_with_many_columns(cuda, n, vocab, dim):
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n + dim)
+    dy = _randn((n, dim), g, cuda)
+    for what, ids in _id_patterns(n, vocab, g, cuda):
+        ids = ids.int()
+        want, err = _grad_want(dy, ids, vocab, 0.5, 2)
+        got = train.EmbeddingGrad(dy, ids, vocab, scale=0.5, padding=2)
+        _near(got, want, err)
+        assert torch.equal(got, train.EmbeddingGrad(dy, ids, vocab, scale=0.5, padding=2)), what
+        _check_rows(train.EmbeddingGradRows(dy, ids, vocab, scale=0.5, padding=2), want, err, ids, 2)
+    train.Check(cuda)
+
+
+@pytest.mark.parametrize("gt", TYPES)
+@pytest.mark.parametrize("n", [3, 900, 2500])
+@pytest.mark.parametrize("dim", [1, 3, 7, 33, 130])
+def test_grad_zeros_between_rows_met(cuda, gt, n, dim):
+    """Zeros for rows in groups of any length, from any start of an output
+    with and without gaps between its rows; nothing outside it is written."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n + dim)
+    vocab = 203
+    dy = _randn((n, dim), g, cuda)
+    ids = torch.randint(0, 12, (n,), generator=g, device=cuda, dtype=torch.int32)
+    ids = torch.where(ids < 9, ids * 13 + 30, ids + 60)
+    want, err = _grad_want(dy, ids, vocab, 1.0, -1)
+    for start, gap in ((0, 0), (1, 0), (5, 0), (3, 2)):
+        buf = torch.full((start + vocab * (dim + gap) + 19,), 9.0, dtype=_dt(gt), device=cuda)
+        out = buf[start:start + vocab * (dim + gap)].view(vocab, dim + gap)[:, :dim]
+        _near(train.EmbeddingGrad(dy, ids, vocab, out=out), want, err)
+        out.fill_(9.0)
+        assert buf.eq(9).all()
