@@ -141,8 +141,12 @@ SIGNATURES = {
                                          _vp, C.c_int, _i64, _vp, _vp]),
     "fg_log_probs": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, C.c_int, _vp, _vp, _vp, _vp,
                                _vp, _vp]),
+    "fg_log_probs_peak": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, C.c_int, _vp, _vp, _vp, _vp,
+                                    _vp, _vp, _vp]),
     "fg_log_probs_grad": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp,
                                     _i64, _vp]),
+    "fg_log_probs_grad_peak": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp,
+                                         _i64, _vp]),
     "fg_clip_grad_norm": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp]),
 }
 

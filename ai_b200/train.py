@@ -175,14 +175,24 @@ def EmbeddingGradRows(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: fl
     return RowsGrad(row_ids, rows, count)
 
 
-class LogProbsResult(NamedTuple):
-    """LogProb, Entropy and LogSum [rows] float32; TopIndex (int32) and
-    TopLogProb [rows, top], None where no alternatives were asked for."""
+class _LogProbsFields(NamedTuple):
     LogProb: torch.Tensor
     Entropy: torch.Tensor
     LogSum: torch.Tensor
     TopIndex: Optional[torch.Tensor]
     TopLogProb: Optional[torch.Tensor]
+
+
+class LogProbsResult(_LogProbsFields):
+    """LogProb, Entropy and LogSum [rows] float32; TopIndex (int32) and
+    TopLogProb [rows, top], None where no alternatives were asked for. Beside
+    these five, Peak [2, rows] float32: every row's largest logit and that
+    one's log probability."""
+    _sums: torch.Tensor  # [5, rows]: the first three, and the peak
+
+    @property
+    def Peak(self) -> torch.Tensor:
+        return self._sums[3:]
 
 
 def _logits(op: str, logits: torch.Tensor, targets: torch.Tensor, scale: float):
@@ -209,27 +219,41 @@ def LogProbs(logits: torch.Tensor, targets: torch.Tensor, scale: float = 1.0, to
     code, logits, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
     if not 0 <= top <= min(width, _lib.MAX_TOP):
         _fail(op, f"{top} alternatives of {width} columns (at most {_lib.MAX_TOP})")
-    out = logits.new_empty((3, rows), dtype=torch.float32)
+    out = logits.new_empty((5, rows), dtype=torch.float32)
     at = out.data_ptr()
     place = value = place_at = value_at = None
     if top:
         place, value = targets.new_empty((rows, top)), out.new_empty((rows, top))
         place_at, value_at = place.data_ptr(), value.data_ptr()
-    _run("fg_log_probs", index, logits.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, top, at,
-         at + 4 * rows, at + 8 * rows, place_at, value_at)
-    return LogProbsResult(*out.unbind(), place, value)
+    _run("fg_log_probs_peak", index, logits.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, top, at,
+         at + 4 * rows, at + 8 * rows, at + 12 * rows, place_at, value_at)
+    logprob, entropy, lse, _, _ = out.unbind()
+    result = LogProbsResult(logprob, entropy, lse, place, value)
+    result._sums = out
+    return result
 
 
-def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, dlogprob: torch.Tensor,
+def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: Optional[torch.Tensor], dlogprob: torch.Tensor,
                  entropy: Optional[torch.Tensor] = None, dentropy: Optional[torch.Tensor] = None,
-                 scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The logits' gradient of ``LogProbs`` from its LogSum (and Entropy) and
-    the gradients of its log probabilities and, where ``dentropy`` is given,
-    of its entropies. ``out`` may be the logits themselves; a new tensor has
-    their rows' distance where that is little more than their length."""
+                 scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                 peak: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The logits' gradient of ``LogProbs`` from its LogSum or its Peak (and
+    Entropy) and the gradients of its log probabilities and, where
+    ``dentropy`` is given, of its entropies. ``out`` may be the logits
+    themselves; a new tensor has their rows' distance where that is little
+    more than their length.
+
+    A LogSum far from 0 has no room in 32 bits for what tells a row's
+    probabilities (for a row of the type's lowest value, or logits with an
+    offset of 1e6): its rounding is a relative error of about 2^-24 |lse| in
+    all of them. With ``peak`` such rows are as exact as others; ``lse`` is not
+    looked at then and may be None."""
     op = "LogProbsGrad"
     code, x, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
-    lse = _float32(op, "lse", lse, rows, index)
+    if peak is None:
+        sums = _float32(op, "lse", lse, rows, index)
+    else:
+        sums = _float32(op, "peak", peak, 2 * rows, index)
     dlogprob = _float32(op, "dlogprob", dlogprob, rows, index)
     entropy_at = dentropy_at = None
     if dentropy is not None:
@@ -250,8 +274,8 @@ def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
         ldo = _stride(out, rows, width)
         if not ldo:
             _fail(op, "out must have contiguous rows")
-    _run("fg_log_probs_grad", index, x.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, lse.data_ptr(),
-         entropy_at, dlogprob.data_ptr(), dentropy_at, out.data_ptr(), ldo)
+    _run("fg_log_probs_grad" if peak is None else "fg_log_probs_grad_peak", index, x.data_ptr(), code, rows, width, ld,
+         targets.data_ptr(), scale, sums.data_ptr(), entropy_at, dlogprob.data_ptr(), dentropy_at, out.data_ptr(), ldo)
     return out
 
 

@@ -58,7 +58,7 @@ def step(table: torch.Tensor, left: torch.Tensor, right: torch.Tensor, temperatu
     sims = cluster.Similarities(a, b)
     p = train.LogProbs(sims, partner, scale=1 / temperature, top=min(top, batch))
     share = torch.full((batch,), -1.0 / batch, device=table.device)
-    dsims = train.LogProbsGrad(sims, partner, p.LogSum, share, scale=1 / temperature)
+    dsims = train.LogProbsGrad(sims, partner, p.LogSum, share, scale=1 / temperature, peak=p.Peak)
     da, db = tensor.MatMul(dsims, b), tensor.MatMul(dsims.t(), a)
     dy = torch.cat([encode_grad(da, a, a_length, a_count, left.shape[1]),
                     encode_grad(db, b, b_length, b_count, right.shape[1])], 1)

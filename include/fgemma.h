@@ -429,14 +429,33 @@ int fg_log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int
                  float scale, int top, float* logprob, float* entropy, float* lse, int32_t* top_index,
                  float* top_logprob, void* stream);
 
+/* The same with one result more, or peak == NULL for none: [2, rows], every
+ * row's largest logit and that one's log probability, which the gradient of
+ * rows far from 0 needs. */
+int fg_log_probs_peak(const void* logits, int dtype, int64_t rows, int64_t width, int64_t ld, const int32_t* targets,
+                      float scale, int top, float* logprob, float* entropy, float* lse, float* peak,
+                      int32_t* top_index, float* top_logprob, void* stream);
+
 /* Its gradient from lse (and entropy) of fg_log_probs and the gradients of
  * logprob and, where dentropy is not NULL, of entropy:
  *   dlogits = scale * (dlogprob * ([j = target] - p) - dentropy * p * (log p + entropy)).
  * A target < 0 has no part of dlogprob; a row of -inf alone has gradient 0.
- * dlogits (row stride ldd) has the logits' type and may be the logits. */
+ * dlogits (row stride ldd) has the logits' type and may be the logits.
+ * p is e^(z - lse) of the lse given, in 32 bits: its relative error is about
+ * 2^-24 |lse|, 1e-5 at a hundred, all of it where the row is a mask of the
+ * type's lowest value; where scale times the largest logit overflows, lse is
+ * -inf and the row counts as empty. For such rows take
+ * fg_log_probs_grad_peak. */
 int fg_log_probs_grad(const void* logits, int dtype, int64_t rows, int64_t width, int64_t ld, const int32_t* targets,
                       float scale, const float* lse, const float* entropy, const float* dlogprob,
                       const float* dentropy, void* dlogits, int64_t ldd, void* stream);
+
+/* The same gradient from the peak of fg_log_probs_peak in place of lse:
+ * log p = scale * (x - peak) + log p(peak), as exact for rows far from 0 as
+ * for others. */
+int fg_log_probs_grad_peak(const void* logits, int dtype, int64_t rows, int64_t width, int64_t ld,
+                           const int32_t* targets, float scale, const float* peak, const float* entropy,
+                           const float* dlogprob, const float* dentropy, void* dlogits, int64_t ldd, void* stream);
 
 /* *norm (device) = the Euclidean norm of all values of `count` contiguous
  * tensors (host arrays of device pointers, sizes and FG_DT_* types), and

@@ -938,3 +938,99 @@ def test_grad_zeros_between_rows_met(cuda, gt, n, dim):
         _near(train.EmbeddingGrad(dy, ids, vocab, out=out), want, err)
         out.fill_(9.0)
         assert buf.eq(9).all()
+
+
+# ------------------------------------------------- forward and gradient together
+def _pair_want(x, t, dl, dh, scale):
+    """(gradient, error bound) of logprob·dl + H·dh in 64 bits from the logits
+    alone. The operators' log p is scale·(x − peak) (two roundings) less log s1
+    (``_sum_error``, its own rounding), their H within ``_check_logprobs``'s."""
+    import torch
+
+    d, logs, mean, _, H, _, empty = _logprobs_want(x, t, scale)
+    fin = lambda v: torch.where(torch.isfinite(v), v, torch.zeros_like(v))  # noqa: E731
+    sums = _sum_error(x.shape[1], fin(H).clamp(min=0)) + 2 * u * fin(logs).abs()
+    H_err = sums * (2 + 3 * fin(mean).abs()) + 2 * u * fin(mean).abs()
+    logp = d - logs[:, None]
+    p = torch.exp(logp)
+    here = p != 0
+    lp_err = torch.where(here, u * (3 * d.abs() + fin(logs).abs()[:, None] + logp.abs()), torch.zeros_like(p)) + sums[:, None]
+    rel = lp_err + u * torch.where(here, logp.abs(), torch.zeros_like(p)) * 2 + 6 * u
+    hit = torch.zeros_like(p)
+    at = torch.arange(len(t), device=x.device)[t >= 0]
+    hit[at, t.long()[t >= 0]] = 1
+    dl = torch.where(t < 0, torch.zeros_like(dl), dl).double()[:, None]
+    want, err = dl * (hit - p), dl.abs() * (p * rel + 2 * u * (hit + p))
+    if dh is not None:
+        dh = dh.double()[:, None]
+        f = torch.where(here, logp + H[:, None], torch.zeros_like(p))
+        want = want - dh * p * f
+        err = err + dh.abs() * p * (f.abs() * (rel + 4 * u) + lp_err + H_err[:, None])
+    zero = torch.zeros_like(want)
+    want = torch.where(empty[:, None], zero, want * scale)
+    err = torch.where(empty[:, None], zero, (err + 3 * u * want.abs() / scale) * scale)
+    # below the exponential's smallest normal result float32 gives 0
+    weights = dl.abs().amax() + (0 if dh is None else dh.abs().amax() * 128)
+    return want, err + scale * 2.0 ** -125 * (weights + 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,pad", [(1, 0), (7, 0), (1000, 0), (1001, 3), (40000, 0)])
+@pytest.mark.parametrize("scale", [1.0, 20.0])
+@pytest.mark.parametrize("with_entropy", [False, True])
+def test_logprobs_pair_of_rows_far_from_zero(cuda, dtype, width, pad, scale, with_entropy):
+    """Rows of the type's lowest value, of one large value, with an offset that
+    leaves lse no room for log s1, beside ordinary and masked ones: the
+    gradient through Peak against 64 bits, from the logits alone."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, width + int(scale))
+    far = 3e4 if dtype == "float16" else 1e6
+    buf = _randn((9, width + pad), g, cuda, "float32") * (3 / scale)
+    buf[0] = torch.finfo(_dt(dtype)).min
+    buf[1] = -6e4 if dtype == "float16" else -1e9
+    buf[2] += far
+    buf[3] -= far
+    buf[4] = -math.inf
+    buf[5, ::2] = torch.finfo(_dt(dtype)).min
+    buf[6, : width // 2] = -math.inf
+    buf[7] = torch.finfo(_dt(dtype)).max
+    buf = buf.to(_dt(dtype))
+    x = buf[:, :width]
+    t = torch.randint(0, width, (9,), generator=g, device=cuda, dtype=torch.int32)
+    t[8] = -1
+    dl = torch.randn(9, generator=g, device=cuda)
+    dh = torch.randn(9, generator=g, device=cuda) if with_entropy else None
+    want, err = _pair_want(x, t, dl, dh, scale)
+    r = train.LogProbs(x, t, scale=scale)
+    assert r.Peak.shape == (2, 9) and torch.equal(r.Peak[0], x.float().amax(1))
+    kept = buf.clone()
+    got = train.LogProbsGrad(x, t, None, dl, entropy=r.Entropy, dentropy=dh, scale=scale, peak=r.Peak)
+    _near(got, want, err)
+    again = train.LogProbsGrad(x, t, r.LogSum, dl, entropy=r.Entropy, dentropy=dh, scale=scale, peak=r.Peak, out=x)
+    assert torch.equal(again, got) and torch.equal(buf[:, width:], kept[:, width:])
+
+
+def test_logprobs_pair_not_finite(cuda):
+    """NaN and +inf reach the gradient through Peak as through LogSum."""
+    import torch
+
+    from ai_b200 import train
+
+    x = torch.zeros(4, 700, device=cuda)
+    x[0, 4] = math.nan
+    x[1, 5] = math.inf
+    x[3] = -math.inf
+    t = torch.zeros(4, dtype=torch.int32, device=cuda)
+    r = train.LogProbs(x, t, top=3)
+    assert r.Peak[0, 1] == math.inf and torch.isnan(r.Peak[:, 0]).all() and r.Peak[:, 3].eq(-math.inf).all()
+    assert float(r.Peak[1, 2]) == float(r.TopLogProb[2, 0]) == float(r.LogProb[2])
+    got = train.LogProbsGrad(x, t, None, torch.ones(4, device=cuda), peak=r.Peak)
+    assert torch.isnan(got[:2]).all() and torch.isfinite(got[2]).all() and not got[3].any()
+    for bad in (r.Peak[0], r.Peak.double(), r.Peak.cpu()):
+        with pytest.raises(train.TensorError):
+            train.LogProbsGrad(x, t, r.LogSum, torch.ones(4, device=cuda), peak=bad)
+    with pytest.raises(train.TensorError):
+        train.LogProbsGrad(x, t, None, torch.ones(4, device=cuda))

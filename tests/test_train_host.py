@@ -124,3 +124,16 @@ def test_python_refuses_host_tensors():
                  lambda: train.ClipGradNorm([], 1.0), lambda: train.ClipGradNorm([x], -1.0)):
         with pytest.raises(train.TensorError):
             call()
+
+
+def test_log_probs_peak_refusals():
+    from ai_b200 import _lib
+
+    for args in ((P, 0, 2, 8, 7, P, 1.0, 0, P, P, P, P, None, None, None),   # stride
+                 (P, 0, 2, 8, 8, P, 1.0, 9, P, P, P, P, P, P, None),         # more alternatives than columns
+                 (P, 0, 2, 8, 8, P, 1.0, 0, P, P, None, P, None, None, None)):  # null
+        assert _call("fg_log_probs_peak", *args) == _lib.FG_EINVAL
+    for args in ((P, 0, 2, 8, 8, P, 1.0, None, P, P, None, P, 8, None),      # no peak
+                 (P, 0, 2, 8, 8, P, 1.0, P, None, P, P, P, 8, None),         # dentropy without entropy
+                 (P, 0, 2, 8, 8, P, 0.0, P, P, P, None, P, 8, None)):
+        assert _call("fg_log_probs_grad_peak", *args) == _lib.FG_EINVAL
