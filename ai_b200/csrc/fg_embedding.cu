@@ -56,14 +56,14 @@ template <typename TW, typename TY, int VEC>
 __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(const TW* __restrict__ table, int64_t vocab, int dim,
                                                                   int64_t ldt, const int32_t* __restrict__ ids,
                                                                   int64_t n, float scale, int padding,
-                                                                  TY* __restrict__ out, int64_t ldo, int* err) {
+                                                                  TY* __restrict__ out, int64_t ldo, int* bad_index) {
   const int64_t t = int64_t(blockIdx.x) * kLookupWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (t >= n) return;
   const int id = ids[t];
   const bool pad = id == padding;
   const bool bad = !pad && (id < 0 || id >= vocab);
-  if (bad && lane == 0) atomicCAS(err, 0, kDevBadIndex);
+  if (bad && lane == 0) *bad_index = 1;
   TY* y = out + t * ldo;
   const int groups = dim / VEC;
   if (pad || bad) {
@@ -101,10 +101,10 @@ constexpr int kSortItems = 16;  // a thread's tokens of a tile
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxDigit = 10;
 
-__device__ __forceinline__ uint32_t token_key(int id, int64_t vocab, int padding, int* err) {
+__device__ __forceinline__ uint32_t token_key(int id, int64_t vocab, int padding, int* bad_index) {
   if (id == padding) return uint32_t(vocab);
   if (id < 0 || id >= vocab) {
-    atomicCAS(err, 0, kDevBadIndex);
+    *bad_index = 1;
     return uint32_t(vocab);
   }
   return uint32_t(id);
@@ -112,14 +112,14 @@ __device__ __forceinline__ uint32_t token_key(int id, int64_t vocab, int padding
 
 // keys of the first pass from the ids (keys == nullptr), else from memory
 __device__ __forceinline__ uint32_t sort_key(const int32_t* ids, const uint32_t* keys, int64_t i, int64_t vocab,
-                                             int padding, int* err) {
-  return keys ? keys[i] : token_key(ids[i], vocab, padding, err);
+                                             int padding, int* bad_index) {
+  return keys ? keys[i] : token_key(ids[i], vocab, padding, bad_index);
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const int32_t* __restrict__ ids,
                                                                  const uint32_t* __restrict__ keys, int64_t n,
                                                                  int64_t vocab, int padding, int shift, int digit_bits,
-                                                                 uint32_t* __restrict__ counts, int* err) {
+                                                                 uint32_t* __restrict__ counts, int* bad_index) {
   __shared__ uint32_t hist[1 << kMaxDigit];
   const int radix = 1 << digit_bits;
   for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const int32_t*
   const int64_t base = int64_t(blockIdx.x) * kSortTile;
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = base + k * kSortThreads + threadIdx.x;
-    if (i < n) atomicAdd(&hist[(sort_key(ids, keys, i, vocab, padding, err) >> shift) & (radix - 1)], 1u);
+    if (i < n) atomicAdd(&hist[(sort_key(ids, keys, i, vocab, padding, bad_index) >> shift) & (radix - 1)], 1u);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < radix; d += kSortThreads) counts[int64_t(d) * gridDim.x + blockIdx.x] = hist[d];
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const int32_t* 
                                                                 int64_t vocab, int padding, int shift, int digit_bits,
                                                                 const uint32_t* __restrict__ counts,
                                                                 uint32_t* __restrict__ keys_out,
-                                                                uint32_t* __restrict__ pos_out, int* err) {
+                                                                uint32_t* __restrict__ pos_out, int* bad_index) {
   constexpr int kWarps = kSortThreads / 32;
   __shared__ uint32_t next[kWarps][1 << kMaxDigit];  // a warp's next place for each digit
   const int radix = 1 << digit_bits;
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const int32_t* 
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = base + 32 * k;
-    key[k] = i < n ? sort_key(ids, keys, i, vocab, padding, err) : 0;
+    key[k] = i < n ? sort_key(ids, keys, i, vocab, padding, bad_index) : 0;
     const unsigned live = __ballot_sync(kFull, i < n);
     rank[k] = 0;
     if (i < n) {
@@ -330,7 +330,7 @@ struct GroupArgs {
   int32_t* row_ids;
   int32_t* count;
   uint32_t* long_runs;  // a count that starts at 0
-  int* err;
+  int* bad_index;
 };
 
 template <int ITEMS>
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) group_kernel(GroupArgs a) {
   }
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k)  // places past the last token sort behind every key
-    mine[k].x = int(mine[k].y) < a.n ? token_key(int(mine[k].x), a.vocab, a.padding, a.err) : 0xffffffffu;
+    mine[k].x = int(mine[k].y) < a.n ? token_key(int(mine[k].x), a.vocab, a.padding, a.bad_index) : 0xffffffffu;
   for (int p = 0; p < a.passes; ++p) {
     const int shift = p * kMaxDigit;
     uint32_t* key_to = a.key[(a.passes - 1 - p) & 1];
@@ -952,7 +952,7 @@ struct FewArgs {
   int64_t token_units, units;
   int32_t* row_ids;  // of the compact gradient
   int32_t* count;
-  int* err;
+  int* bad_index;
 };
 
 size_t few_shared(int words, int slots) { return size_t(words) * 32 * 4 + size_t(words) * 4 + size_t(slots) * 12; }
@@ -978,7 +978,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(FewArgs a, const TY* _
     slot_count[i] = 0;
   }
   for (int i = tid; i < a.words * 32; i += kFewThreads) {
-    const uint32_t key = i < a.n ? token_key(a.ids[i], a.vocab, a.padding, a.err) : uint32_t(a.vocab);
+    const uint32_t key = i < a.n ? token_key(a.ids[i], a.vocab, a.padding, a.bad_index) : uint32_t(a.vocab);
     keys[i] = key < a.vocab ? key : kNoKey;
   }
   __syncthreads();
@@ -1125,8 +1125,8 @@ struct Scratch {
 int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids, int64_t n, int64_t vocab, int64_t dim,
                    float scale, int padding, void* grad, int grad_dtype, int64_t ldg, int accumulate, int32_t* row_ids,
                    int32_t* count, cudaStream_t s) {
-  int* err = nullptr;
-  FG_TRY(device_error_word(&err));
+  int* bad_index = nullptr;
+  FG_TRY(device_index_word(&bad_index));
   const bool compact = count != nullptr;
   if (compact && n == 0) {
     FG_CUDA_TRY(cudaMemsetAsync(count, 0, sizeof(int32_t), s));
@@ -1154,7 +1154,7 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     f.units = f.token_units + (compact || accumulate ? 0 : blocks_of(vocab, 32) * (wide ? slices : 1));
     f.row_ids = row_ids;
     f.count = count;
-    f.err = err;
+    f.bad_index = bad_index;
     // no more blocks than run at once: each makes the table again
     const unsigned blocks = unsigned(std::min<int64_t>(blocks_of(f.units, kFewWarps), int64_t(sm_count()) * kFewBlocks));
     const size_t shared = few_shared(f.words, f.slots);
@@ -1224,16 +1224,16 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
   }
   if (n > 0 && grouped_here) {
     GroupArgs g{ids, int(n), vocab, padding, passes, counts, {key[0], key[1]}, {pos[0], pos[1]}, zeros_first ? nullptr : met,
-                compact ? place : nullptr, row_ids, count, long_runs, err};
+                compact ? place : nullptr, row_ids, count, long_runs, bad_index};
     FG_TRY(group_tokens(g, s));
   } else if (n > 0) {
     FG_CUDA_TRY(cudaMemsetAsync(long_runs, 0, sizeof(uint32_t), s));
     for (int p = 0; p < passes; ++p) {
       const uint32_t* k = p ? key[(p + 1) & 1] : nullptr;
-      sort_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, n, vocab, padding, p * digit, digit, counts, err);
+      sort_count_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, n, vocab, padding, p * digit, digit, counts, bad_index);
       scan_kernel<<<1, kScanThreads, 0, s>>>(counts, tiles << digit, nullptr);
       sort_move_kernel<<<unsigned(tiles), kSortThreads, 0, s>>>(ids, k, p ? pos[(p + 1) & 1] : nullptr, n, vocab, padding,
-                                                               p * digit, digit, counts, key[p & 1], pos[p & 1], err);
+                                                               p * digit, digit, counts, key[p & 1], pos[p & 1], bad_index);
     }
   }
   a.keys = key[grouped_here ? 0 : (passes - 1) & 1];
@@ -1314,8 +1314,8 @@ int fg_embedding(const void* table, int table_dtype, int64_t vocab, int64_t dim,
   if (n == 0) return FG_OK;
   if (!ids || !out || (!table && vocab > 0)) return set_error(FG_EINVAL, "fg_embedding: null operand");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int* err = nullptr;
-  FG_TRY(device_error_word(&err));
+  int* bad_index = nullptr;
+  FG_TRY(device_index_word(&bad_index));
   const unsigned blocks = unsigned(blocks_of(n, kLookupWarps));
   const bool wide = grouped(table, table_dtype, dim, ldt, 4) && grouped(out, out_dtype, dim, ldo, 4);
   return by_dtype(table_dtype, [&](auto tw) {
@@ -1325,9 +1325,9 @@ int fg_embedding(const void* table, int table_dtype, int64_t vocab, int64_t dim,
       const TW* w = static_cast<const TW*>(table);
       TY* y = static_cast<TY*>(out);
       if (wide)
-        lookup_kernel<TW, TY, 4><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, err);
+        lookup_kernel<TW, TY, 4><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, bad_index);
       else
-        lookup_kernel<TW, TY, 1><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, err);
+        lookup_kernel<TW, TY, 1><<<blocks, kLookupWarps * 32, 0, s>>>(w, vocab, int(dim), ldt, ids, n, scale, padding, y, ldo, bad_index);
       FG_CUDA_TRY(cudaGetLastError());
       return FG_OK;
     });

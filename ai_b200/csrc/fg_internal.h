@@ -62,6 +62,11 @@ class OncePerDevice {
 // recorded timeout into FG_ETIMEOUT, resetting the word.
 int device_error_word(int** out);
 int check_device_error_word();
+// The block's word that a kernel sets to 1 when it skips a token id or a
+// target outside its range, and its check (after a synchronisation): FG_EINVAL
+// where it was set, resetting it.
+int device_index_word(int** out);
+int check_device_index_word();
 // Registers another status block of device `dev` (the no-allocation entry
 // point's static one) for check_device_error_word and the wait limit.
 int register_status_block(int dev, int* block);

@@ -109,7 +109,7 @@ struct LogProbsArgs {
   float* peak;  // [2, rows] or null: the largest logit, its log probability
   int32_t* top_index;
   float* top_logprob;
-  int* err;
+  int* bad_index;
 };
 
 // The sums of a part of a row about a reference, its largest entry:
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     if (t < a.width)
       xt = widen(x[t]);
     else
-      atomicCAS(a.err, 0, kDevBadIndex);
+      *a.bad_index = 1;
   }
   RowSums sums{-INFINITY, 0.f, 0.f};
   float lost1 = 0.f, lost2 = 0.f;  // what rounding added to the sums too much
@@ -552,7 +552,7 @@ struct LogProbsGradArgs {
   const float* entropy;
   const float* dlogprob;
   const float* dentropy;
-  int* err;
+  int* bad_index;
 };
 
 // Elementwise: a warp takes kGradGroups 16-byte groups a lane of one row, all
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kGradWarps * 32) logprobs_grad_kernel(LogProbs
     }
   }
   const int t = a.targets[row];
-  if (t >= a.width && part == 0 && lane == 0) atomicCAS(a.err, 0, kDevBadIndex);
+  if (t >= a.width && part == 0 && lane == 0) *a.bad_index = 1;
   const bool none = t < 0 || t >= a.width;
   const float ref = PEAK ? a.peak[row] : a.lse[row];
   const float peak_logprob = PEAK ? a.peak_logprob[row] : 0.f;
@@ -674,7 +674,7 @@ int log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int64_
     return set_error(FG_EINVAL, "fg_log_probs: null operand");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   LogProbsArgs a{rows, ld, int(width), top, targets, scale, logprob, entropy, lse, peak, top_index, top_logprob, nullptr};
-  FG_TRY(device_error_word(&a.err));
+  FG_TRY(device_index_word(&a.bad_index));
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     const T* x = static_cast<const T*>(logits);
@@ -711,7 +711,7 @@ int log_probs_grad(const void* logits, int dtype, int64_t rows, int64_t width, i
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   LogProbsGradArgs a{rows, ld, ldd, int(width), targets, scale, lse, peak, peak ? peak + rows : nullptr,
                      entropy, dlogprob, dentropy, nullptr};
-  FG_TRY(device_error_word(&a.err));
+  FG_TRY(device_index_word(&a.bad_index));
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     return launch_logprobs_grad(a, static_cast<const T*>(logits), static_cast<T*>(dlogits), s);

@@ -26,7 +26,6 @@ enum DeviceError : int {
   kDevTimeoutAccEmpty = 4,  // MMA waited too long for the epilogue
   kDevTimeoutDrain = 5,     // teardown waited too long for in-flight work
   kDevBadArgs = 6,          // a kernel saw arguments it cannot handle
-  kDevBadIndex = 7,         // a token id or a target outside its range (reported as FG_EINVAL)
 };
 
 // Default limit of a pipeline wait, and the fixed limit of the teardown
@@ -34,12 +33,14 @@ enum DeviceError : int {
 constexpr uint64_t kWaitTimeoutNs = 2000ull * 1000ull * 1000ull;  // 2 s
 
 // The per-device status block kernels receive as `int* gerr`: the error
-// word first, then the pipeline-wait limit in nanoseconds (set from the
-// host, fg_set_wait_limit). 16 bytes, zero error and kWaitTimeoutNs when
-// created.
+// word first, then a word of its own for indices out of range (read by
+// fg_synchronize alone, so that one operator's bad id neither hides a wait
+// that gave up nor fails another call), then the pipeline-wait limit in
+// nanoseconds (set from the host, fg_set_wait_limit). 16 bytes, zeros and
+// kWaitTimeoutNs when created.
 struct DeviceStatus {
   int err;
-  int reserved;
+  int bad_index;
   unsigned long long wait_limit_ns;
 };
 static_assert(sizeof(DeviceStatus) == 16, "status block layout");

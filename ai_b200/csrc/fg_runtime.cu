@@ -1,13 +1,13 @@
 // Library runtime: thread-local error messages, device queries, the
 // per-device status block kernels report bounded-wait timeouts into (and
 // read their wait limit from), and the device-memory helpers of the C ABI.
+#include <cstddef>
 #include <mutex>
 #include <vector>
 
 #include <atomic>
 
 #include "fg_internal.h"
-#include "fg_ptx.cuh"
 
 namespace fg {
 
@@ -23,7 +23,7 @@ std::vector<cudaMemPool_t> g_pools;  // per device: op-level scratch
 // Host image of the device status block (fg_ptx.cuh DeviceStatus).
 struct DeviceStatusHost {
   int err;
-  int reserved;
+  int bad_index;
   unsigned long long wait_limit_ns;
 };
 constexpr unsigned long long kDefaultWaitLimitNs = 2000ull * 1000ull * 1000ull;
@@ -110,10 +110,32 @@ int check_device_error_word() {
       if (!first) first = v;
     }
   }
-  if (first == kDevBadIndex)
-    return set_error(FG_EINVAL, "a token id or a target was outside its range (kernel status %d)", first);
   if (first) return set_error(FG_ETIMEOUT, "a device wait gave up (kernel status %d)", first);
   return FG_OK;
+}
+
+int device_index_word(int** out) {
+  FG_TRY(device_error_word(out));
+  *out += offsetof(DeviceStatusHost, bad_index) / sizeof(int);
+  return FG_OK;
+}
+
+int check_device_index_word() {
+  int dev = 0;
+  FG_CUDA_TRY(cudaGetDevice(&dev));
+  char* block = nullptr;
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (int(g_dev_err.size()) > dev) block = reinterpret_cast<char*>(g_dev_err[dev]);
+  }
+  if (!block) return FG_OK;
+  int* word = reinterpret_cast<int*>(block + offsetof(DeviceStatusHost, bad_index));
+  int v = 0;
+  FG_CUDA_TRY(cudaMemcpy(&v, word, sizeof(int), cudaMemcpyDeviceToHost));
+  if (v == 0) return FG_OK;
+  const int zero = 0;
+  FG_CUDA_TRY(cudaMemcpy(word, &zero, sizeof(int), cudaMemcpyHostToDevice));
+  return set_error(FG_EINVAL, "a token id or a target was outside its range");
 }
 
 int set_wait_limit(int dev, unsigned long long ns) {
@@ -239,7 +261,8 @@ int fg_memcpy_d2h(int device, void* dst, const void* src, int64_t bytes) {
 
 int fg_synchronize(int device) {
   FG_CUDA_TRY(cudaSetDevice(device));
-  return fg::check_device_error_word();
+  FG_TRY(fg::check_device_error_word());
+  return fg::check_device_index_word();
 }
 
 int fg_set_wait_limit(int device, int64_t nanoseconds) {

@@ -132,7 +132,9 @@ int fg_memcpy_h2d(int device, void* dst, const void* src, int64_t bytes);
 int fg_memcpy_d2h(int device, void* dst, const void* src, int64_t bytes);
 /* Waits for all work on `device`; returns FG_ETIMEOUT (and clears the
  * record) when a kernel's bounded wait gave up since the last check, and
- * FG_EINVAL when a training operator met an id or a target out of range. */
+ * FG_EINVAL (and clears that record) when a training operator met an id or a
+ * target out of range. Where both happened, this call reports the wait and
+ * the next one the id; no other call reports an id. */
 int fg_synchronize(int device);
 /* Limit, in nanoseconds, of every pipeline wait (mbarrier) inside the
  * library's kernels on `device`; 0 restores the default of 2 s. A wait that

@@ -1034,3 +1034,76 @@ def test_logprobs_pair_not_finite(cuda):
             train.LogProbsGrad(x, t, r.LogSum, torch.ones(4, device=cuda), peak=bad)
     with pytest.raises(train.TensorError):
         train.LogProbsGrad(x, t, None, torch.ones(4, device=cuda))
+
+
+# --------------------------------------------- what an id out of range touches
+def _bad_id(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    train.Embedding(torch.ones(6, 8, device=cuda), torch.tensor([9], dtype=torch.int32, device=cuda))
+
+
+def _check_reports_once(cuda):
+    from ai_b200 import _lib, train
+
+    with pytest.raises(_lib.FGError) as e:
+        train.Check(cuda)
+    assert e.value.code == _lib.FG_EINVAL
+    train.Check(cuda)
+
+
+def test_bad_id_leaves_other_calls_alone(cuda):
+    """KMeans and a model's forward with good inputs succeed after it, and the
+    report is still there for Check."""
+    import torch
+
+    from ai_b200 import cluster, gemma
+    from ai_b200 import synthetic as S
+
+    x = _randn((300, 16), _gen(cuda, 9), cuda)
+    _bad_id(cuda)
+    cluster.KMeans(x, 3, 4, 1)
+    _check_reports_once(cuda)
+    cfg = S.small_config(layers=1, vocab=256)
+    model = gemma.from_synthetic(cfg, S.make_weights(cfg, seed=0), device=0, max_batch_tokens=256)
+    try:
+        ids, lengths = S.make_ids(2, 16, 1, cfg["vocab_size"]), torch.full((2,), 16, dtype=torch.int32).numpy()
+        _bad_id(cuda)
+        model.embed_padded(ids, lengths)
+        model.check()
+        _check_reports_once(cuda)
+    finally:
+        model.close()
+
+
+@pytest.mark.parametrize("noalloc", [False, True])
+def test_bad_id_does_not_hide_a_wait_that_gave_up(cuda, noalloc):
+    """A bad id, then a product whose waits run out under a limit of 1 us: the
+    timeout is reported first, then the id."""
+    import torch
+
+    from ai_b200 import _lib
+
+    lib = _lib.lib()
+    fn = lib.fg_matmul_noalloc if noalloc else lib.fg_matmul
+    g = _gen(cuda, 5)
+    m, n, k = 512, 512, 8192
+    a, w, out = _randn((m, k), g, cuda), _randn((n, k), g, cuda), torch.empty(m, n, device=cuda)
+
+    def product():
+        _lib.check(fn(m, n, k, a.data_ptr(), k, w.data_ptr(), k, 1, out.data_ptr(), n, None, _lib.PREC_TF32,
+                      torch.cuda.current_stream().cuda_stream))
+
+    product()  # set-up before the limit changes
+    _lib.check(lib.fg_synchronize(0))
+    try:
+        _bad_id(cuda)
+        _lib.check(lib.fg_set_wait_limit(0, 1000))
+        product()
+        rc = lib.fg_synchronize(0)
+    finally:
+        _lib.check(lib.fg_set_wait_limit(0, 0))
+    assert rc == _lib.FG_ETIMEOUT
+    _check_reports_once(cuda)
