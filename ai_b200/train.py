@@ -188,11 +188,12 @@ class LogProbsResult(_LogProbsFields):
     TopLogProb [rows, top], None where no alternatives were asked for. Beside
     these five, Peak [2, rows] float32: every row's largest logit and that
     one's log probability."""
-    _sums: torch.Tensor  # [5, rows]: the first three, and the peak
+    _sums: torch.Tensor  # [3, rows], the first three; the peak lies between its first two rows
 
     @property
     def Peak(self) -> torch.Tensor:
-        return self._sums[3:]
+        rows = self._sums.shape[1]
+        return self._sums.as_strided((2, rows), (rows, 1), self._sums.storage_offset() + rows)
 
 
 def _logits(op: str, logits: torch.Tensor, targets: torch.Tensor, scale: float):
@@ -219,16 +220,16 @@ def LogProbs(logits: torch.Tensor, targets: torch.Tensor, scale: float = 1.0, to
     code, logits, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
     if not 0 <= top <= min(width, _lib.MAX_TOP):
         _fail(op, f"{top} alternatives of {width} columns (at most {_lib.MAX_TOP})")
-    out = logits.new_empty((5, rows), dtype=torch.float32)
+    # three rows with room for two between them: one allocation, and three views in one call
+    out = logits.new_empty_strided((3, rows), (3 * rows, 1), dtype=torch.float32)
     at = out.data_ptr()
     place = value = place_at = value_at = None
     if top:
         place, value = targets.new_empty((rows, top)), out.new_empty((rows, top))
         place_at, value_at = place.data_ptr(), value.data_ptr()
     _run("fg_log_probs_peak", index, logits.data_ptr(), code, rows, width, ld, targets.data_ptr(), scale, top, at,
-         at + 4 * rows, at + 8 * rows, at + 12 * rows, place_at, value_at)
-    logprob, entropy, lse, _, _ = out.unbind()
-    result = LogProbsResult(logprob, entropy, lse, place, value)
+         at + 12 * rows, at + 24 * rows, at + 4 * rows, place_at, value_at)
+    result = LogProbsResult(*out.unbind(), place, value)
     result._sums = out
     return result
 

@@ -1107,3 +1107,21 @@ def test_bad_id_does_not_hide_a_wait_that_gave_up(cuda, noalloc):
         _lib.check(lib.fg_set_wait_limit(0, 0))
     assert rc == _lib.FG_ETIMEOUT
     _check_reports_once(cuda)
+
+
+def test_logprobs_results_lie_apart(cuda):
+    """Peak and the three sums share an allocation and nothing else."""
+    import torch
+
+    from ai_b200 import train
+
+    for rows in (0, 1, 5, 1000):
+        x = _randn((rows, 9), _gen(cuda, rows), cuda)
+        r = train.LogProbs(x, torch.zeros(rows, dtype=torch.int32, device=cuda))
+        parts = [r.LogProb, r.Entropy, r.LogSum, r.Peak[0], r.Peak[1]]
+        assert r.Peak.shape == (2, rows) and r.Peak.is_contiguous() and all(p.is_contiguous() and p.shape == (rows,) for p in parts)
+        at = sorted((p.data_ptr(), p.data_ptr() + 4 * rows) for p in parts)
+        assert rows == 0 or all(a[1] <= b[0] for a, b in zip(at, at[1:]))
+        assert torch.equal(r.Peak[0], x.amax(1)) if rows else True
+        want = x.double().logsumexp(1) if rows else x.double().sum(1)
+        assert torch.allclose(r.LogSum.double(), want, rtol=1e-5, atol=1e-6)
