@@ -2,6 +2,8 @@
 //
 //   N = sqrt(Σ_i ‖g_i‖²),  out_i = c·g_i,  c = max_norm / N if max_norm < N < ∞, else 1
 //
+// N < ∞ is asked of the float32 that the caller gets, so that what it reads and
+// what was done agree.
 // Two passes over memory: a block sums the squares of its share of equal
 // pieces and leaves one partial sum; every block of the second pass adds all
 // partial sums in one order, so all have the same c, and scales its share,
@@ -16,6 +18,7 @@
 // The tensors' addresses travel in the kernel's arguments: no copy to the
 // device, whatever their number.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "fg_internal.h"
@@ -128,15 +131,18 @@ __device__ __forceinline__ double squares(const T* x, int n) {
   return sum;
 }
 
-template <typename T>
-__device__ __forceinline__ void scale_piece(const T* x, T* y, int n, float c) {
+// C: float, or double for a factor below float's normal numbers, which has
+// lost bits as a float.
+template <typename T, typename C>
+__device__ __forceinline__ void scale_piece(const T* x, T* y, int n, C c) {
   constexpr int V = 16 / int(sizeof(T));
+  constexpr int kAheadOf = sizeof(C) == 4 ? 4 : 1;
   const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  for_groups<4>(
+  for_groups<kAheadOf>(
       x, n,
       [&](int i, auto& p) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.set(j, p.get(j) * c);
+        for (int j = 0; j < V; ++j) p.set(j, float(p.get(j) * c));
         if (alike) {
           p.store(y + i);
         } else {
@@ -144,7 +150,18 @@ __device__ __forceinline__ void scale_piece(const T* x, T* y, int n, float c) {
           for (int j = 0; j < V; ++j) y[i + j] = p.v[j];
         }
       },
-      [&](int i) { y[i] = narrow<T>(widen(x[i]) * c); });
+      [&](int i) { y[i] = narrow<T>(float(widen(x[i]) * c)); });
+}
+
+// Piece `at` of a tensor, n of its values.
+template <int N, typename C>
+__device__ __forceinline__ void scale_any(const TensorList<N>& t, int i, int64_t at, int n, C c) {
+  if (t.dtype[i] == FG_DT_F32)
+    scale_piece(static_cast<const float*>(t.in[i]) + at, static_cast<float*>(t.out[i]) + at, n, c);
+  else if (t.dtype[i] == FG_DT_BF16)
+    scale_piece(static_cast<const __nv_bfloat16*>(t.in[i]) + at, static_cast<__nv_bfloat16*>(t.out[i]) + at, n, c);
+  else
+    scale_piece(static_cast<const __half*>(t.in[i]) + at, static_cast<__half*>(t.out[i]) + at, n, c);
 }
 
 template <int N>
@@ -176,19 +193,19 @@ __global__ void __launch_bounds__(kNormThreads, 4) clip_kernel(const __grid_cons
   for (int i = threadIdx.x; i < partials; i += kNormThreads) s += __ldcg(partial + i);
   const double total = sqrt(block_sum(s, shared));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = float(total);
-  const bool clips = total > double(max_norm) && isfinite(total);
-  const float c = clips ? float(double(max_norm) / total) : 1.f;
+  const bool clips = total > double(max_norm) && isfinite(float(total));
+  const double factor = clips ? double(max_norm) / total : 1.0;
+  const float c = float(factor);
+  const bool small = factor > 0.0 && c < FLT_MIN;
   for (int piece = t.first[t.count] - 1 - blockIdx.x; piece >= 0; piece -= gridDim.x) {
     const int i = tensor_of(t, piece);
     if (!clips && t.in[i] == t.out[i]) continue;
     const int64_t at = int64_t(piece - t.first[i]) * kPiece;
     const int n = int(min(int64_t(kPiece), t.size[i] - at));
-    if (t.dtype[i] == FG_DT_F32)
-      scale_piece(static_cast<const float*>(t.in[i]) + at, static_cast<float*>(t.out[i]) + at, n, c);
-    else if (t.dtype[i] == FG_DT_BF16)
-      scale_piece(static_cast<const __nv_bfloat16*>(t.in[i]) + at, static_cast<__nv_bfloat16*>(t.out[i]) + at, n, c);
+    if (small)
+      scale_any(t, i, at, n, factor);
     else
-      scale_piece(static_cast<const __half*>(t.in[i]) + at, static_cast<__half*>(t.out[i]) + at, n, c);
+      scale_any(t, i, at, n, c);
   }
 }
 

@@ -462,8 +462,8 @@ int fg_log_probs_grad_peak(const void* logits, int dtype, int64_t rows, int64_t 
 /* *norm (device) = the Euclidean norm of all values of `count` contiguous
  * tensors (host arrays of device pointers, sizes and FG_DT_* types), and
  * outs[i] = grads[i] * max_norm / norm where max_norm < norm < inf, else
- * outs[i] = grads[i] (a norm that is not finite clips nothing: the caller
- * reads it and skips its step). outs NULL = in place; outs[i] may be
+ * outs[i] = grads[i] (a norm that is not finite as the float32 that *norm
+ * holds clips nothing: the caller reads it and skips its step). outs NULL = in place; outs[i] may be
  * grads[i]. max_norm may be +inf: the norm alone. The arrays are read
  * during the call only. */
 int fg_clip_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,

@@ -1125,3 +1125,40 @@ def test_logprobs_results_lie_apart(cuda):
         assert torch.equal(r.Peak[0], x.amax(1)) if rows else True
         want = x.double().logsumexp(1) if rows else x.double().sum(1)
         assert torch.allclose(r.LogSum.double(), want, rtol=1e-5, atol=1e-6)
+
+
+# ------------------------------------------------ norms at the ends of the range
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("value,count,max_norm", [
+    (1e38, 1000, 1.0),       # a norm of 3.2e39: inf as a float32
+    (3e38, 2, 1e-3),         # 4.2e38
+    (1.6e38, 4, 1e-3),       # 3.2e38: finite, the factor 3e-42
+    (1.6e38, 4, 1e-30),      # the factor 3e-69
+    (2.0 ** 126, 16, 2.0 ** -20),
+    (1e37, 30011, 7.0),
+    (1e20, 70000, 1e-25),
+])
+def test_clip_of_the_largest_norms(cuda, dtype, value, count, max_norm):
+    """A norm that is not finite as returned changes nothing; a finite one
+    clips within one rounding however small the factor."""
+    import torch
+
+    from ai_b200 import train
+
+    x = torch.full((count,), value, device=cuda).to(_dt(dtype))
+    x[::3] *= -0.5
+    kept = x.clone()
+    norm = math.sqrt(float((x.double() ** 2).sum()))
+    as_float = float(torch.tensor(norm, dtype=torch.float64).float())
+    out = torch.empty_like(x)
+    got = float(train.ClipGradNorm([x], max_norm, out=[out]))
+    assert torch.equal(x, kept)
+    assert float(train.ClipGradNorm([x], max_norm)) == got
+    assert torch.equal(x, out)
+    if math.isinf(as_float):
+        assert got == math.inf and torch.equal(x, kept)
+        return
+    assert abs(got / norm - 1) <= 4 * u
+    m32 = float(torch.tensor(max_norm, dtype=torch.float32))
+    want = kept.double() * (m32 / norm)
+    _near(x, want, 4 * u * want.abs())
