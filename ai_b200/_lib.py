@@ -33,6 +33,7 @@ DT_F16 = 2
 
 MAX_DENSE = 4
 MAX_TOP = 64  # FG_MAX_TOP: alternatives of fg_log_probs
+MAX_SCALE = 2.3e38  # its largest scale: that times log2 e is a float32
 
 # Phases of fg_model_read_profile (include/fgemma.h FG_PHASE_*).
 PHASES = ["embed", "gemm_qkv", "qk_norm_rope", "attention", "gemm_o", "residual",

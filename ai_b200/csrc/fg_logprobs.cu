@@ -98,11 +98,27 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
+// Differences of entries times the scale. Below a scale of 1 the entries are
+// halved first: their difference may lie past float's range and its product
+// within it. (Above 1 such a product lies past it too.) The factors are pairs
+// in the kernel's arguments, where they take no registers (made in the kernel,
+// up to 12 registers spilled: 8192 x 8192 with 64 alternatives 143 -> 150 us).
+struct Scaled {
+  float2 half, log2;  // ½ or 1; the scale over it, times log2 e
+  float scale;        // the scale over it
+  explicit Scaled(float s) : scale(s < 1.f ? 2.f * s : s) {
+    half.x = half.y = s < 1.f ? 0.5f : 1.f;
+    log2.x = log2.y = scale * kLog2e;
+  }
+  __device__ __forceinline__ float difference(float x, float ref) const { return fmaf(x, half.x, -half.x * ref); }
+};
+
 struct LogProbsArgs {
   int64_t rows, ld;
   int width, top;
   const int32_t* targets;
   float scale;
+  Scaled k;
   float* logprob;
   float* entropy;
   float* lse;
@@ -112,18 +128,18 @@ struct LogProbsArgs {
   int* bad_index;
 };
 
-// The sums of a part of a row about a reference, its largest entry:
-// s1 = Σ e^(scale·(x − ref)), s2 = Σ e^(scale·(x − ref))·(x − ref). While
-// s1 is 0, nothing above −∞ has been met and the reference says nothing.
+// The sums of a part of a row about a reference, its largest entry, with
+// t = log2(e^(scale·(x − ref))): s1 = Σ 2^t, s2 = Σ 2^t·t. While s1 is 0,
+// nothing above −∞ has been met and the reference says nothing.
 struct RowSums {
   float ref, s1, s2;
 
-  // the same sums about another reference; k = scale·log2 e
-  __device__ __forceinline__ void move(float to, float k) {
-    const float d = ref - to;
+  // the same sums about another reference
+  __device__ __forceinline__ void move(float to, const Scaled& k) {
+    const float t = k.difference(ref, to) * k.log2.x;
     ref = to;
-    const float c = s1 == 0.f ? 0.f : ex2_approx(d * k);
-    s2 = c == 0.f ? 0.f : c * fmaf(d, s1, s2);
+    const float c = s1 == 0.f ? 0.f : ex2_approx(t);
+    s2 = c == 0.f ? 0.f : c * fmaf(t, s1, s2);
     s1 = c == 0.f ? 0.f : c * s1;
   }
 };
@@ -149,7 +165,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 // The sums of all lanes together, in every lane. A lane that has met nothing
 // above −∞ has the reference −∞ and sums of 0.
-__device__ __forceinline__ RowSums warp_join(RowSums v, float k) {
+__device__ __forceinline__ RowSums warp_join(RowSums v, const Scaled& k) {
   v.move(warp_max_nan(v.ref), k);
   v.s1 = warp_sum(v.s1);
   v.s2 = warp_sum(v.s2);
@@ -301,7 +317,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   const int skip = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int tiles = (a.width + skip + kTile - 1) / kTile;
   const int step = WARPS * split;
-  const float k = a.scale * kLog2e;
+  const Scaled& k = a.k;
   // column of a lane's entry i of a tile
   auto column = [&](int tile, int i) { return tile * kTile + (i / V) * (32 * V) + lane * V - skip + i % V; };
 
@@ -374,15 +390,14 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     }
     const float ref = sums.ref == -INFINITY ? 0.f : sums.ref;
     float2 s1 = make_float2(0.f, 0.f), s2 = s1;
-    const float2 minus = make_float2(-ref, -ref), k2 = make_float2(k, k);
+    const float2 minus = make_float2(-k.half.x * ref, -k.half.x * ref);
 #pragma unroll
     for (int i = 0; i < kItems; i += 2) {
-      float2 d = add2(make_float2(v[i], v[i + 1]), minus);
-      d = make_float2(max_nan(d.x, -FLT_MAX), max_nan(d.y, -FLT_MAX));  // −∞ times e^−∞ = 0 would be no number
-      float2 e = mul2(d, k2);
-      e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+      float2 t = mul2(fma2(make_float2(v[i], v[i + 1]), k.half, minus), k.log2);
+      t = make_float2(max_nan(t.x, -FLT_MAX), max_nan(t.y, -FLT_MAX));  // −∞ times 2^−∞ = 0 would be no number
+      const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
       s1 = add2(s1, e);
-      s2 = fma2(e, d, s2);
+      s2 = fma2(e, t, s2);
     }
     add_kept(sums.s1, lost1, s1.x + s1.y);
     add_kept(sums.s2, lost2, s2.x + s2.y);
@@ -479,10 +494,11 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
   }
   const bool empty = sums.s1 == 0.f;
   const float ref = empty ? 0.f : sums.ref, logs = logf(sums.s1);
+  auto log_prob = [&](float x) { return empty ? -INFINITY : fmaf(k.difference(x, ref), k.scale, -logs); };
   if (threadIdx.x == 0) {
     const bool skipped = t < 0 || t >= a.width;
-    a.logprob[row] = skipped ? 0.f : empty ? -INFINITY : fmaf(xt - ref, a.scale, -logs);
-    a.entropy[row] = empty ? 0.f : logs - a.scale * (sums.s2 / sums.s1);
+    a.logprob[row] = skipped ? 0.f : log_prob(xt);
+    a.entropy[row] = empty ? 0.f : logs - kLn2 * (sums.s2 / sums.s1);
     a.lse[row] = fmaf(ref, a.scale, logs);
     if (a.peak) {
       a.peak[row] = sums.ref;
@@ -496,7 +512,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS)
     if (warp > 0 || i >= a.top) return;
     const uint64_t key = list.key[n];
     a.top_index[row * a.top + i] = int32_t(rank_index(key));
-    a.top_logprob[row * a.top + i] = empty ? -INFINITY : fmaf(rank_value(uint32_t(key >> 32)) - ref, a.scale, -logs);
+    a.top_logprob[row * a.top + i] = log_prob(rank_value(uint32_t(key >> 32)));
   }
 }
 
@@ -546,6 +562,7 @@ struct LogProbsGradArgs {
   int width;
   const int32_t* targets;
   float scale;
+  Scaled k;
   const float* lse;  // or the peak and its log probability
   const float* peak;
   const float* peak_logprob;
@@ -593,6 +610,7 @@ __global__ void __launch_bounds__(kGradWarps * 32) logprobs_grad_kernel(LogProbs
   const bool none = t < 0 || t >= a.width;
   const float ref = PEAK ? a.peak[row] : a.lse[row];
   const float peak_logprob = PEAK ? a.peak_logprob[row] : 0.f;
+  const Scaled& k = a.k;
   const float g0 = none ? 0.f : a.dlogprob[row];
   const bool empty = ref == -INFINITY;
   float h = 0.f, H = 0.f;
@@ -609,7 +627,7 @@ __global__ void __launch_bounds__(kGradWarps * 32) logprobs_grad_kernel(LogProbs
     for (int i = 0; i < V; ++i) {
       // the product with lse rounded as it is in lse, so that the largest entry
       // of a row that has all the probability has exactly 1
-      const float lp = PEAK ? fmaf(in[g].get(i) - ref, a.scale, peak_logprob)
+      const float lp = PEAK ? fmaf(k.difference(in[g].get(i), ref), k.scale, peak_logprob)
                             : __fsub_rn(__fmul_rn(in[g].get(i), a.scale), ref);
       const float p = ex2_approx(lp * kLog2e);
       float d = g0 * ((j + i == t ? 1.f : 0.f) - p);
@@ -667,13 +685,14 @@ int log_probs(const void* logits, int dtype, int64_t rows, int64_t width, int64_
   if (!known_dtype(dtype)) return set_error(FG_EINVAL, "fg_log_probs: unknown element type %d", dtype);
   if (ld < width) return set_error(FG_EINVAL, "fg_log_probs: leading dimension smaller than the row");
   if (!(scale > 0.f) || std::isinf(scale)) return set_error(FG_EINVAL, "fg_log_probs: scale must be positive and finite");
+  if (std::isinf(scale * kLog2e)) return set_error(FG_EINVAL, "fg_log_probs: scale %g is too large", double(scale));
   if (top < 0 || top > kMaxTop || top > width)
     return set_error(FG_EINVAL, "fg_log_probs: %d alternatives of %lld columns (at most %d)", top, (long long)width, kMaxTop);
   if (rows == 0) return FG_OK;
   if (!logits || !targets || !logprob || !entropy || !lse || (top > 0 && (!top_index || !top_logprob)))
     return set_error(FG_EINVAL, "fg_log_probs: null operand");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  LogProbsArgs a{rows, ld, int(width), top, targets, scale, logprob, entropy, lse, peak, top_index, top_logprob, nullptr};
+  LogProbsArgs a{rows, ld, int(width), top, targets, scale, Scaled(scale), logprob, entropy, lse, peak, top_index, top_logprob, nullptr};
   FG_TRY(device_index_word(&a.bad_index));
   return by_dtype(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
@@ -709,7 +728,7 @@ int log_probs_grad(const void* logits, int dtype, int64_t rows, int64_t width, i
   if (!logits || !targets || (!lse && !peak) || !dlogprob || !dlogits || (dentropy && !entropy))
     return set_error(FG_EINVAL, "fg_log_probs_grad: null operand");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  LogProbsGradArgs a{rows, ld, ldd, int(width), targets, scale, lse, peak, peak ? peak + rows : nullptr,
+  LogProbsGradArgs a{rows, ld, ldd, int(width), targets, scale, Scaled(scale), lse, peak, peak ? peak + rows : nullptr,
                      entropy, dlogprob, dentropy, nullptr};
   FG_TRY(device_index_word(&a.bad_index));
   return by_dtype(dtype, [&](auto tag) {

@@ -218,6 +218,8 @@ def LogProbs(logits: torch.Tensor, targets: torch.Tensor, scale: float = 1.0, to
     probable columns (equal logits by ascending index)."""
     op = "LogProbs"
     code, logits, ld, targets, rows, width, index = _logits(op, logits, targets, scale)
+    if scale > _lib.MAX_SCALE:
+        _fail(op, f"scale {scale} is too large")
     if not 0 <= top <= min(width, _lib.MAX_TOP):
         _fail(op, f"{top} alternatives of {width} columns (at most {_lib.MAX_TOP})")
     # three rows with room for two between them: one allocation, and three views in one call

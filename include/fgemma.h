@@ -419,7 +419,8 @@ int fg_embedding_grad_rows(const void* dy, int dy_dtype, int64_t ldy, const int3
                            int64_t ldr, int32_t* count, void* stream);
 
 /* Log probabilities over rows of logits [rows, width] (row stride ld), with
- * z = scale * logits (scale > 0, an inverse temperature):
+ * z = scale * logits (an inverse temperature: scale > 0, scale * log2 e finite
+ * in 32 bits):
  *   logprob[r] = log softmax(z_r)[targets[r]] (0 where targets[r] < 0),
  *   entropy[r] = -sum p log p, lse[r] = log sum e^z (for the gradient),
  * and the `top` (at most 64) most probable columns of every row in

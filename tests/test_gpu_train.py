@@ -1162,3 +1162,63 @@ def test_clip_of_the_largest_norms(cuda, dtype, value, count, max_norm):
     m32 = float(torch.tensor(max_norm, dtype=torch.float32))
     want = kept.double() * (m32 / norm)
     _near(x, want, 4 * u * want.abs())
+
+
+# ----------------------------------------------- scales at the ends of the range
+def _fits(v, dtype="float32"):
+    """64-bit values as the type has them at its ends: infinite past them."""
+    import torch
+
+    return torch.where(torch.isinf(v.to(_dt(dtype))), torch.sign(v) * math.inf, v)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("width,top", [(8, 0), (9, 5), (3000, 20), (70000, 3)])
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 2e-37, 1e-30, 0.5, 1e30, 2e38])
+def test_logprobs_of_any_scale(cuda, dtype, width, top, scale):
+    """Masked entries have no probability at any scale, and differences past
+    float32's range count by what the scale makes of them."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, width)
+    most = float(torch.finfo(_dt(dtype)).max)
+    near = max(min(1 / scale, most / 8), 1e-30)
+    x = _randn((5, width), g, cuda, "float32") * near
+    x[1, ::2] = -math.inf
+    x[2] = torch.where(x[2] > 0, 0.9 * most, -0.9 * most)
+    x[3, ::2] = -most
+    x[4] = -math.inf
+    x = x.to(_dt(dtype))
+    t = torch.randint(0, width, (5,), generator=g, device=cuda, dtype=torch.int32)
+    s32 = float(torch.tensor(scale, dtype=torch.float32))
+    r = train.LogProbs(x, t, scale=scale, top=top)
+    d, logs, mean, logp, H, lse, empty = _logprobs_want(x, t, s32)
+    fin = lambda v: torch.where(torch.isfinite(v), v, torch.zeros_like(v))  # noqa: E731
+    tol = _sum_error(width, fin(H).clamp(min=0)) + u * fin(logs).abs() * 2
+    dt = fin(d.gather(1, t.long()[:, None])[:, 0])
+    _near(r.LogProb, _fits(logp), tol + u * (3 * dt.abs() + fin(logp).abs()))
+    _near(r.LogSum, _fits(lse), tol + u * (fin(lse) - fin(logs)).abs() * 2)
+    _near(r.Entropy, H, tol * (2 + 3 * fin(mean).abs()) + 2 * u * fin(mean).abs())
+    if top:
+        _, index = x.float().sort(dim=1, descending=True, stable=True)
+        assert torch.equal(r.TopIndex.long(), index[:, :top])
+        dk = d.gather(1, index[:, :top])
+        want = torch.where(empty[:, None], torch.full_like(dk, -math.inf), dk - logs[:, None])
+        _near(r.TopLogProb, _fits(want), tol[:, None] + u * (3 * fin(dk).abs() + fin(want).abs()))
+    if scale > 1e-40:  # a gradient of that scale is below float32's numbers
+        dl, dh = torch.randn(5, generator=g, device=cuda), torch.randn(5, generator=g, device=cuda)
+        want, err = _pair_want(x, t, dl, dh, s32)
+        got = train.LogProbsGrad(x, t, None, dl, entropy=r.Entropy, dentropy=dh, scale=scale, peak=r.Peak)
+        _near(got, _fits(want, dtype), err + 2.0 ** -149)
+
+
+def test_logprobs_refuses_a_scale_too_large(cuda):
+    import torch
+
+    from ai_b200 import train
+
+    x, t = torch.zeros(2, 4, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
+    with pytest.raises(train.TensorError):
+        train.LogProbs(x, t, scale=3e38)
