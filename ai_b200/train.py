@@ -78,10 +78,16 @@ def _rows(t: torch.Tensor, rows: int, cols: int):
 
 
 def Check(device=None) -> None:
-    """Waits for the device's work and raises what its kernels reported: an
-    id or a target out of range (status FG_EINVAL)."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    _lib.check(_lib.lib().fg_synchronize(index))
+    """Waits for the work of a device (the current one where none or "cuda" is
+    given) and raises what its kernels reported: an id or a target out of
+    range (status FG_EINVAL). The current device stays what it is."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        _fail("Check", f"{device} is not a CUDA device")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    with torch.cuda.device(index):  # fg_synchronize makes its device the current one
+        rc = _lib.lib().fg_synchronize(index)
+    _lib.check(rc)
 
 
 def Embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding: int = -1,

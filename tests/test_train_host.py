@@ -137,3 +137,53 @@ def test_log_probs_peak_refusals():
                  (P, 0, 2, 8, 8, P, 1.0, P, None, P, P, P, 8, None),         # dentropy without entropy
                  (P, 0, 2, 8, 8, P, 0.0, P, P, P, None, P, 8, None)):
         assert _call("fg_log_probs_grad_peak", *args) == _lib.FG_EINVAL
+
+
+@pytest.mark.parametrize("current,device,want", [(0, None, 0), (1, None, 1), (1, "cuda", 1), (0, "cuda:1", 1), (1, "cuda:0", 0), (0, 2, 2)])
+def test_check_waits_for_the_device_asked_for_and_goes_back(monkeypatch, current, device, want):
+    """"cuda" is the current device, and the caller's current device is the
+    same afterwards although fg_synchronize makes its own current; also where
+    it reports an id."""
+    import torch
+
+    from ai_b200 import _lib, train
+
+    state = {"current": current, "asked": [], "rc": 0}
+
+    class Library:
+        @staticmethod
+        def fg_synchronize(index):
+            state["asked"].append(index)
+            state["current"] = index
+            return state["rc"]
+
+        @staticmethod
+        def fg_last_error():
+            return b"an id"
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["current"] = state["current"], self.index
+
+        def __exit__(self, *exc):
+            state["current"] = self.before
+
+    monkeypatch.setattr(_lib, "lib", lambda: Library)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    train.Check(device)
+    assert state["asked"] == [want] and state["current"] == current
+    state["rc"] = _lib.FG_EINVAL
+    with pytest.raises(_lib.FGError):
+        train.Check(device)
+    assert state["asked"] == [want] * 2 and state["current"] == current
+
+
+def test_check_refuses_a_host_device():
+    from ai_b200 import train
+
+    with pytest.raises(train.TensorError):
+        train.Check("cpu")
