@@ -288,13 +288,28 @@ def LogProbsGrad(logits: torch.Tensor, targets: torch.Tensor, lse: Optional[torc
     return out
 
 
+def _packed(grads: Sequence[torch.Tensor]) -> Optional[list]:
+    """The gradients with packed copies of those whose rows lie apart, None
+    where one has no such rows."""
+    got = []
+    for g in grads:
+        if not g.is_contiguous():
+            if g.dim() != 2 or not _stride(g, *g.shape):
+                return None
+            g = g.contiguous()
+        got.append(g)
+    return got
+
+
 def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
                  out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """The Euclidean norm of all gradients together (a float32 scalar on
     their device), and every gradient times max_norm / norm where the norm is
     finite and larger: in place, or into the tensors of ``out``. A norm that
-    is not finite changes nothing. The tensors are contiguous and on one
-    device; their types may differ."""
+    is not finite changes nothing. The tensors are on one device and
+    contiguous, or matrices with rows apart (as ``LogProbsGrad`` has for padded
+    logits), which go through a packed copy; their types may differ. Those of
+    ``out`` are contiguous."""
     op = "ClipGradNorm"
     if not max_norm >= 0:
         _fail(op, f"max_norm {max_norm} must be at least 0")
@@ -307,12 +322,13 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
         types = list(map(_TYPE_OF, grads))
         codes = list(map(_DTYPES.__getitem__, types))
         index = grads[0].get_device()
-        alike = index >= 0 and set(map(T.get_device, grads)) == {index} and all(map(T.is_contiguous, grads))
+        alike = index >= 0 and set(map(T.get_device, grads)) == {index}
+        packed = grads if all(map(T.is_contiguous, grads)) else _packed(grads)
         sizes = list(map(T.numel, grads))
     except (KeyError, AttributeError, TypeError):
         _fail(op, "gradients must be float32, bfloat16 or float16 tensors")
-    if not alike:
-        _fail(op, "gradients must be contiguous tensors on one CUDA device")
+    if not alike or packed is None:
+        _fail(op, "gradients must be tensors on one CUDA device, contiguous or matrices with rows apart")
     outs = outs_at = None
     if out is not None:
         if len(out) != n or list(map(_TYPE_OF, out)) != types or list(map(T.numel, out)) != sizes or \
@@ -320,8 +336,12 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
             _fail(op, "out must match the gradients' sizes, types and device, contiguous")
         outs = array("Q", map(T.data_ptr, out))
         outs_at = outs.buffer_info()[0]
-    ins, sizes, codes = array("Q", map(T.data_ptr, grads)), array("q", sizes), array("i", codes)
+    ins, sizes, codes = array("Q", map(T.data_ptr, packed)), array("q", sizes), array("i", codes)
     norm = grads[0].new_empty((), dtype=torch.float32)
     _run("fg_clip_grad_norm", index, n, ins.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], outs_at,
          max_norm, norm.data_ptr())
+    if packed is not grads and out is None:
+        for g, p in zip(grads, packed):
+            if p is not g:
+                g.copy_(p)
     return norm

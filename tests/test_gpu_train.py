@@ -1222,3 +1222,41 @@ def test_logprobs_refuses_a_scale_too_large(cuda):
     x, t = torch.zeros(2, 4, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
     with pytest.raises(train.TensorError):
         train.LogProbs(x, t, scale=3e38)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("max_norm", [1e-3, 1e6])
+def test_clip_of_a_padded_gradient(cuda, dtype, max_norm):
+    """The gradient of padded logits has their layout; it clips as a packed one
+    does, alone and among others, and what lies between its rows stays."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 21)
+    x = _randn((30, 107), g, cuda, dtype)[:, :100]
+    t = torch.randint(0, 100, (30,), generator=g, device=cuda, dtype=torch.int32)
+    r = train.LogProbs(x, t)
+    d = train.LogProbsGrad(x, t, r.LogSum, torch.ones(30, device=cuda))
+    assert not d.is_contiguous()
+    buf = torch.full((30, 107), 9.0, device=cuda, dtype=_dt(dtype))
+    rows = buf[:, :100]
+    rows.copy_(d)
+    other = _randn((50,), g, cuda)
+    for with_other in (False, True):
+        def among(a, b):
+            return [b, a] if with_other else [a]
+
+        rows.copy_(d)
+        packed, b1, b2, b3 = d.contiguous(), other.clone(), other.clone(), other.clone()
+        want = float(train.ClipGradNorm(among(packed, b1), max_norm))
+        out = among(torch.empty_like(packed), torch.empty_like(b2))
+        assert float(train.ClipGradNorm(among(rows, b2), max_norm, out=out)) == want
+        assert torch.equal(rows, d) and torch.equal(b2, other)
+        assert all(torch.equal(a, b) for a, b in zip(out, among(packed, b1)))
+        assert float(train.ClipGradNorm(among(rows, b3), max_norm)) == want
+        assert torch.equal(rows, packed) and torch.equal(b3, b1) and buf[:, 100:].eq(9).all()
+    with pytest.raises(train.TensorError):
+        train.ClipGradNorm([d.t()], 1.0)
+    with pytest.raises(train.TensorError):
+        train.ClipGradNorm([d.contiguous()], 1.0, out=[rows])
