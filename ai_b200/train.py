@@ -57,6 +57,12 @@ def _int32(op: str, name: str, t: torch.Tensor, index: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _padding(op: str, padding: int) -> int:
+    if not -2 ** 31 <= padding < 2 ** 31:  # the call would take its lower 32 bits
+        _fail(op, f"padding {padding} is not an int32")
+    return padding
+
+
 def _float32(op: str, name: str, t: torch.Tensor, rows: int, index: int) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != index or t.numel() != rows:
         _fail(op, f"{name} must be {rows} float32 values on cuda:{index}")
@@ -110,8 +116,8 @@ def Embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, paddin
     ids = _int32(op, "ids", ids, index)
     table, ld = _rows(table, vocab, dim)
     out = table.new_empty((*ids.shape, dim), dtype=dtype)
-    _run("fg_embedding", index, table.data_ptr(), code, vocab, dim, ld, ids.data_ptr(), ids.numel(), scale, padding,
-         out.data_ptr(), out_code, dim)
+    _run("fg_embedding", index, table.data_ptr(), code, vocab, dim, ld, ids.data_ptr(), ids.numel(), scale,
+         _padding(op, padding), out.data_ptr(), out_code, dim)
     return out
 
 
@@ -155,8 +161,8 @@ def EmbeddingGrad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
         ldo = _stride(out, vocab, dim)
         if not ldo:
             _fail(op, "out must have contiguous rows")
-    _run("fg_embedding_grad", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding,
-         out.data_ptr(), _DTYPES[out.dtype], ldo, int(accumulate))
+    _run("fg_embedding_grad", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale,
+         _padding(op, padding), out.data_ptr(), _DTYPES[out.dtype], ldo, int(accumulate))
     return out
 
 
@@ -176,8 +182,8 @@ def EmbeddingGradRows(dy: torch.Tensor, ids: torch.Tensor, vocab: int, scale: fl
     code, dy, ld, ids, n, dim, index = _grad_args(op, dy, ids, vocab, dtype)
     row_ids, count = ids.new_empty(n), ids.new_empty(1)
     rows = dy.new_empty((n, dim), dtype=dtype)
-    _run("fg_embedding_grad_rows", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale, padding,
-         row_ids.data_ptr(), rows.data_ptr(), _DTYPES[rows.dtype], dim, count.data_ptr())
+    _run("fg_embedding_grad_rows", index, dy.data_ptr(), code, ld, ids.data_ptr(), n, vocab, dim, scale,
+         _padding(op, padding), row_ids.data_ptr(), rows.data_ptr(), _DTYPES[rows.dtype], dim, count.data_ptr())
     return RowsGrad(row_ids, rows, count)
 
 

@@ -1260,3 +1260,19 @@ def test_clip_of_a_padded_gradient(cuda, dtype, max_norm):
         train.ClipGradNorm([d.t()], 1.0)
     with pytest.raises(train.TensorError):
         train.ClipGradNorm([d.contiguous()], 1.0, out=[rows])
+
+
+@pytest.mark.parametrize("padding", [2 ** 31, 2 ** 32, -2 ** 31 - 1, 2 ** 40 + 3])
+def test_a_padding_that_is_no_id_is_refused(cuda, padding):
+    """A padding past int32 named another id's rows by its lower bits."""
+    import torch
+
+    from ai_b200 import train
+
+    x, i = torch.ones(4, 8, device=cuda), torch.zeros(4, dtype=torch.int32, device=cuda)
+    for call in (lambda: train.Embedding(x, i, padding=padding), lambda: train.EmbeddingGrad(x, i, 4, padding=padding),
+                 lambda: train.EmbeddingGradRows(x, i, 4, padding=padding)):
+        with pytest.raises(train.TensorError):
+            call()
+    for padding in (2 ** 31 - 1, -2 ** 31):
+        assert train.Embedding(x, i, padding=padding).eq(1).all()
