@@ -1276,3 +1276,174 @@ def test_a_padding_that_is_no_id_is_refused(cuda, padding):
             call()
     for padding in (2 ** 31 - 1, -2 ** 31):
         assert train.Embedding(x, i, padding=padding).eq(1).all()
+
+
+# ------------------------------------------- reports, captures, streams, long sums
+@pytest.mark.parametrize("n,vocab,dim", [(600, 50, 16), (5000, 300, 33), (20000, 262144, 96), (300000, 1000, 4)])
+def test_gradients_skip_and_report_ids_out_of_range(cuda, n, vocab, dim):
+    """One launch, a cluster's sort, zeros beside it, tiles through memory: ids
+    past the table and negative ones leave no trace but the report."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, n)
+    dy = _randn((n, dim), g, cuda)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int32)
+    ids[::7], ids[1::11], ids[2::13], ids[3::17] = vocab, -1, -2 ** 31, 2 ** 31 - 1
+    good = (ids >= 0) & (ids < vocab)
+    kept = torch.where(good, ids, torch.full_like(ids, -5))
+    want, err = _grad_want(dy, kept, vocab, 1.0, -5)
+    got = train.EmbeddingGrad(dy, ids, vocab, padding=-5)
+    _check_reports_once(cuda)
+    _near(got, want, err)
+    r = train.EmbeddingGradRows(dy, ids, vocab, padding=-5)
+    _check_reports_once(cuda)
+    _check_rows(r, want, err, kept, -5)
+    old = torch.ones(vocab, dim, device=cuda)
+    new = train.EmbeddingGrad(dy, ids, vocab, padding=-5, out=old.clone(), accumulate=True)
+    _check_reports_once(cuda)
+    _near(new, want + 1, err + u * (want.abs() + (want + 1).abs()))
+
+
+@pytest.mark.parametrize("width,rows", [(9, 4), (700, 3), (70000, 2)])
+def test_targets_out_of_range_are_reported(cuda, width, rows):
+    """A target past the row counts as none, forward and back."""
+    import torch
+
+    from ai_b200 import train
+
+    x = _randn((rows, width), _gen(cuda, width), cuda)
+    good = torch.full((rows,), -1, dtype=torch.int32, device=cuda)
+    one = torch.ones(rows, device=cuda)
+    want = train.LogProbs(x, good)
+    dwant = train.LogProbsGrad(x, good, want.LogSum, one, entropy=want.Entropy, dentropy=one)
+    dpeak = train.LogProbsGrad(x, good, None, one, entropy=want.Entropy, dentropy=one, peak=want.Peak)
+    train.Check(cuda)
+    for bad in (width, 2 ** 31 - 1):
+        t = good.clone()
+        t[-1] = bad
+        got = train.LogProbs(x, t)
+        _check_reports_once(cuda)
+        assert all(torch.equal(a, b) for a, b in zip(got[:3], want[:3])) and not got.LogProb.any()
+        d = train.LogProbsGrad(x, t, want.LogSum, one, entropy=want.Entropy, dentropy=one)
+        _check_reports_once(cuda)
+        assert torch.equal(d, dwant)
+        d = train.LogProbsGrad(x, t, None, one, entropy=want.Entropy, dentropy=one, peak=want.Peak)
+        _check_reports_once(cuda)
+        assert torch.equal(d, dpeak)
+
+
+def test_large_table_gradient_in_a_graph(cuda):
+    """The zeros that are written beside the sort, the marks before both and the
+    tiled sort, captured once and replayed on new ids."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 14)
+    vocab, dim, n, many = 262144, 96, 20000, 270000
+    dy, dy2 = _randn((n, dim), g, cuda), _randn((many, 4), g, cuda)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=cuda, dtype=torch.int32)
+    ids2 = torch.randint(0, 5000, (many,), generator=g, device=cuda, dtype=torch.int32)
+
+    def both():
+        return [train.EmbeddingGrad(dy, ids, vocab, scale=0.5), train.EmbeddingGrad(dy2, ids2, 5000),
+                *train.EmbeddingGradRows(dy2, ids2, 5000)]
+
+    side = torch.cuda.Stream(cuda)
+    with torch.cuda.stream(side):
+        both()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = both()
+    for low in (1, 100, vocab // 2):
+        ids.copy_(torch.randint(0, low, (n,), generator=g, device=cuda, dtype=torch.int32))
+        ids2.copy_(torch.randint(0, min(low, 5000), (many,), generator=g, device=cuda, dtype=torch.int32))
+        for o in outs:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, err = _grad_want(dy, ids, vocab, 0.5, -1)
+        _near(outs[0], want, err)
+        for a, b in zip([o.clone() for o in outs], both()):
+            assert torch.equal(a, b)
+
+
+def test_operators_on_two_streams_at_once(cuda):
+    """Calls in flight together share the pool that their scratch comes from,
+    and no part of it."""
+    import torch
+
+    from ai_b200 import train
+
+    g = _gen(cuda, 15)
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    data = []
+    for n, vocab, dim in ((60000, 262144, 64), (280000, 3000, 24)):
+        dy = _randn((n, dim), g, cuda)
+        ids = (vocab ** torch.rand(n, generator=g, device=cuda, dtype=torch.float64)).int().clamp(0, vocab - 1)
+        data.append((dy, ids, vocab, train.EmbeddingGrad(dy, ids, vocab), train.EmbeddingGradRows(dy, ids, vocab),
+                     train.ClipGradNorm([dy.clone()], 1.0)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            dy, ids, vocab = data[i][:3]
+            with torch.cuda.stream(s):
+                got[i].append((train.EmbeddingGrad(dy, ids, vocab), train.EmbeddingGradRows(dy, ids, vocab),
+                               train.ClipGradNorm([dy], math.inf)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for dense, rows, norm in got[i]:
+            assert torch.equal(dense, data[i][3]) and torch.equal(norm, data[i][5])
+            assert all(torch.equal(a, b) for a, b in zip(rows, data[i][4]))
+
+
+def _tight(width, H, logs):
+    """What the kernel's sums may be off by, relative: a term's exponent 4u·|d|
+    and its exponential 4u as in ``_sum_error``; 8 additions and one in a tile,
+    the tiles' compensated sum 3, the lanes 5, warps and blocks of a row 10; a
+    lane's running maximum moves at most 8 times (a term's own rounding 2u, the
+    factor's exponential 4u and two products)."""
+    return u * (4 * H + 4 + 9 + 3 + 5 + 10 + 8 * 8) + 2 * u * abs(logs)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(1, 262144), (40, 262144), (3400, 30011)])
+def test_logprobs_long_sums(cuda, dtype, rows, width):
+    import torch
+
+    from ai_b200 import train
+
+    x = _randn((rows, width), _gen(cuda, rows), cuda, dtype)
+    r = train.LogProbs(x, torch.zeros(rows, dtype=torch.int32, device=cuda))
+    for i in sorted({0, rows // 2, rows - 1}):
+        _, logs, mean, logp, H, lse, _ = _logprobs_want(x[i:i + 1], torch.zeros(1, dtype=torch.int32, device=cuda), 1.0)
+        tol = _tight(width, float(H), float(logs))
+        assert abs(float(r.LogSum[i]) - float(lse)) <= tol + u * (abs(float(lse)) + 2 * abs(float(lse - logs)))
+        assert abs(float(r.LogProb[i]) - float(logp)) <= tol + 2 * u * abs(float(logp))
+        assert abs(float(r.Entropy[i]) - float(H)) <= tol * (2 + 3 * abs(float(mean))) + 2 * u * abs(float(mean)) + u * float(H)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_logprobs_small_terms_beside_large_ones(cuda, dtype):
+    """512 entries of 0, then many whose sum in a tile is below half the last
+    bit of a lane's running sum: together 180 of its rounding errors, lost if
+    tiles were added without compensation."""
+    import torch
+
+    from ai_b200 import train
+
+    rows, width = 3400, 100003
+    x = torch.full((rows, width), -16.75, device=cuda, dtype=_dt(dtype))
+    x[:, :512] = 0
+    r = train.LogProbs(x, torch.zeros(rows, dtype=torch.int32, device=cuda))
+    s1 = 512 + (width - 512) * math.exp(-16.75)
+    H = math.log(s1) + (width - 512) * math.exp(-16.75) * 16.75 / s1
+    tol = u * (4 * H + 4 + 9 + 3 + 5) + 2 * u * math.log(s1)
+    lost = math.log(s1 / 512)
+    assert lost > 1.5 * tol
+    assert float((r.LogSum.double() - math.log(s1)).abs().max()) <= tol
+    assert float((r.LogProb.double() + math.log(s1)).abs().max()) <= tol
