@@ -5,8 +5,8 @@
 //   lookup:   y[t] = scale · W[id_t]
 //   gradient: G[v] = scale · Σ_{t : id_t = v} dy[t]
 //
-// Up to 2048 tokens the gradient is one launch whose blocks group the tokens in
-// a hash table each. More are sorted by id, stably, so a row's tokens stay in
+// Few tokens' gradient (up to 2048, of not too many columns) is one launch whose
+// blocks group the tokens in a hash table each. Others are sorted by id, stably, so a row's tokens stay in
 // their order (within one cluster up to 262144, through memory beyond), and
 // cut into chunks of equal length however often a token occurs; the runs of
 // one id are summed in registers, and those longer than a chunk joined in a
@@ -929,14 +929,14 @@ __global__ void __launch_bounds__(kSumWarps * 32) join_kernel(SumArgs a, TG* gra
 // that the work grows with tokens^2 x slices: up to kFewWork of that, beyond it
 // the order of ids is cheaper. A call, here and sorted: 1024 x 1024 bf16 14.6
 // and 20.8 us, rows met 18.7 and 23.2 (8M); 1500 x 512 20.8 and 21.2, 25.1 and
-// 24.0 (9M); 1024 x 301 fp32 18.0 and 20.9, 21.0 and 24.8 (10M); 1500 x 768
+// 24.0 (9M: the rows met are even there, and one limit does for both); 1024 x 301 fp32 18.0 and 20.9, 21.0 and 24.8 (10M); 1500 x 768
 // bf16 23.0 and 21.3, 32.6 and 23.3 (13M); 2048 x 1023 fp32 105 and 25, 168
 // and 35 (128M).
 constexpr int kFewTokens = 2048;
 constexpr int64_t kFewWork = 10 << 20;
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewBlocks = 4;  // an SM's
+constexpr int kFewBlocks = 4;  // launched for an SM
 constexpr int kFewRing = 8;
 constexpr int kWholeRun = 32;  // tokens of a run that one warp sums
 constexpr uint32_t kNoKey = 0xffffffffu;
@@ -1155,7 +1155,10 @@ int embedding_grad(const void* dy, int dy_dtype, int64_t ldy, const int32_t* ids
     f.row_ids = row_ids;
     f.count = count;
     f.bad_index = bad_index;
-    // no more blocks than run at once: each makes the table again
+    // Each block makes the table again, so no more than about what runs at once:
+    // four an SM with 16-bit gradients or single columns and up to 1024 tokens;
+    // three fit from there on (their tables take 57 KB), two where fp32 gradients
+    // go in fours (128 registers), and the rest of a full grid follows them.
     const unsigned blocks = unsigned(std::min<int64_t>(blocks_of(f.units, kFewWarps), int64_t(sm_count()) * kFewBlocks));
     const size_t shared = few_shared(f.words, f.slots);
     return by_dtype(grad_dtype, [&](auto tg) {

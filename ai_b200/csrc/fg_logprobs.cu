@@ -14,10 +14,10 @@
 // A row whose entries are all −∞ has log probabilities −∞, entropy 0 and
 // gradient 0; a row with a NaN or a +∞ has NaN in all of them.
 //
-// Bound by memory without alternatives: 8192 x 8192 fp32 in 44 us, 6.1 TB/s
-// (bf16 35 us, 3.9 TB/s: instructions, 165 of a warp a tile of 512). The
+// Bound by memory without alternatives: 8192 x 8192 fp32 in 43 us, 6.2 TB/s
+// (bf16 34 us, 3.9 TB/s: instructions, 165 of a warp a tile of 512). The
 // alternatives cost instructions: 8 of them 63 us, 64 of them 140. One row of
-// 262144 bf16 with 20 of them 17.8 us a call (its kernel 14.5 when profiled,
+// 262144 bf16 with 20 of them 18.4 us a call (its kernel 14.5 when profiled,
 // from cold caches). The gradient is elementwise: 8192 x 8192 fp32 in 83 us, 6.5 TB/s.
 #include <cooperative_groups.h>
 
@@ -575,8 +575,7 @@ struct LogProbsGradArgs {
 // Elementwise: a warp takes kGradGroups 16-byte groups a lane of one row, all
 // loaded before the first is used; groups are those of the logits' memory,
 // stored whole where the gradient's lie alike. PEAK: log p from the row's peak,
-// else from lse (8192 x 8192 from cold caches, peak and lse: fp32 88 and 86 us,
-// bf16 65.5 and 65.5).
+// else from lse (8192 x 8192, peak and lse: fp32 85 and 83 us, bf16 61 and 60).
 constexpr int kGradWarps = 8;
 constexpr int kGradGroups = 4;
 
