@@ -347,7 +347,8 @@ def ClipGradNorm(grads: Sequence[torch.Tensor], max_norm: float,
     _run("fg_clip_grad_norm", index, n, ins.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], outs_at,
          max_norm, norm.data_ptr())
     if packed is not grads and out is None:
-        for g, p in zip(grads, packed):
-            if p is not g:
-                g.copy_(p)
+        with torch.no_grad():
+            for g, p in zip(grads, packed):
+                if p is not g:
+                    g.copy_(p)
     return norm

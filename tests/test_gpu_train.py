@@ -1447,3 +1447,17 @@ def test_logprobs_small_terms_beside_large_ones(cuda, dtype):
     assert lost > 1.5 * tol
     assert float((r.LogSum.double() - math.log(s1)).abs().max()) <= tol
     assert float((r.LogProb.double() + math.log(s1)).abs().max()) <= tol
+
+
+def test_clip_of_tensors_that_require_gradients(cuda):
+    """Clipped alike whether their rows lie apart or not."""
+    import torch
+
+    from ai_b200 import train
+
+    whole = _randn((20, 30), _gen(cuda, 3), cuda)
+    apart = torch.zeros(20, 33, device=cuda)[:, :30].requires_grad_()
+    apart.data.copy_(whole)
+    whole.requires_grad_()
+    assert float(train.ClipGradNorm([whole], 0.5)) == float(train.ClipGradNorm([apart], 0.5))
+    assert torch.equal(whole, apart)
